@@ -216,6 +216,94 @@ int32_t fa_decode_paged(const fa_paged_params* p, void* stream) {
   return fa::launch_decode_paged(*p, static_cast<cudaStream_t>(stream));
 }
 
+int32_t fa_paged_plan(const fa_paged_plan_params* p, void* stream) {
+  fa::NvtxRange r("fa_paged_plan");
+  if (p == nullptr) return fa::set_error(FA_ERR_INVALID_ARGUMENT, "params is NULL");
+  if (p->batch <= 0 || p->max_blocks <= 0 || p->num_blocks <= 0 || p->num_tokens < 0)
+    return fa::set_error(FA_ERR_INVALID_ARGUMENT, "plan: batch, block table width and blocks must be positive");
+  if (p->batch > FA_PLAN_MAX_BATCH)
+    return fa::set_error(FA_ERR_UNSUPPORTED, "plan: at most %d requests", FA_PLAN_MAX_BATCH);
+  if (p->block_size <= 0 || (p->block_size & (p->block_size - 1)))
+    return fa::set_error(FA_ERR_INVALID_ARGUMENT, "paged cache block size must be a power of two");
+  if (p->context_lens == nullptr || p->new_lens == nullptr || p->block_table == nullptr || p->free_blocks == nullptr ||
+      p->free_count == nullptr || (p->slot_mapping == nullptr && p->num_tokens > 0) || p->cu_seqlens == nullptr ||
+      p->context_lens_out == nullptr || p->free_count_out == nullptr)
+    return fa::set_error(FA_ERR_INVALID_ARGUMENT, "plan: no pointer may be NULL");
+  if (p->batch > 1 && p->bt_stride < p->max_blocks)
+    return fa::set_error(FA_ERR_INVALID_ARGUMENT, "plan: rows of the block table must not overlap");
+  return fa::launch_paged_plan(*p, static_cast<cudaStream_t>(stream));
+}
+
+namespace {
+bool cache_rows_ok(const void* ptr, const int64_t (&st)[4], int num_blocks, int block_size, int heads) {
+  const int n[3] = {num_blocks, block_size, heads};
+  if (st[3] != 1 || reinterpret_cast<uintptr_t>(ptr) % 16) return false;
+  for (int i = 0; i < 3; ++i)
+    if (n[i] > 1 && (st[i] <= 0 || st[i] % 16)) return false;
+  return true;
+}
+
+// What the 8-bit cache kernels rely on; `rows16` are the 16-bit tensors (strides with unit inner stride last).
+int check_cache8(int dtype, int cache_dtype, int heads_kv, int head_dim, int num_blocks, int block_size,
+                 const void* k, const int64_t (&ks)[4], const void* v, const int64_t (&vs)[4]) {
+  if (dtype != FA_F16 && dtype != FA_BF16)
+    return fa::set_error(FA_ERR_INVALID_ARGUMENT, "8-bit cache: the 16-bit tensors must be float16 or bfloat16");
+  if (cache_dtype != FA_CACHE_E4M3 && cache_dtype != FA_CACHE_INT8)
+    return fa::set_error(FA_ERR_INVALID_ARGUMENT, "8-bit cache: the cache must be float8_e4m3fn or int8");
+  if (heads_kv <= 0 || num_blocks <= 0 || block_size <= 0 || (block_size & (block_size - 1)))
+    return fa::set_error(FA_ERR_INVALID_ARGUMENT, "8-bit cache: heads and blocks must be positive, the block size a power of two");
+  if (head_dim <= 0 || head_dim > 256 || head_dim % 16)
+    return fa::set_error(FA_ERR_UNSUPPORTED, "8-bit cache: head_dim must be a multiple of 16 up to 256, got %d", head_dim);
+  if (!cache_rows_ok(k, ks, num_blocks, block_size, heads_kv) || !cache_rows_ok(v, vs, num_blocks, block_size, heads_kv))
+    return fa::set_error(FA_ERR_UNSUPPORTED, "8-bit cache: caches need unit inner stride and rows on 16-byte boundaries");
+  return 0;
+}
+
+bool rows16_ok(const void* ptr, const int64_t (&st)[3], int64_t n0, int64_t n1) {
+  return st[2] == 1 && reinterpret_cast<uintptr_t>(ptr) % 16 == 0 && (n0 <= 1 || st[0] % 8 == 0) && (n1 <= 1 || st[1] % 8 == 0);
+}
+}  // namespace
+
+int32_t fa_paged8_append(const fa_paged8_append_params* p, void* stream) {
+  fa::NvtxRange r("fa_paged8_append");
+  if (p == nullptr) return fa::set_error(FA_ERR_INVALID_ARGUMENT, "params is NULL");
+  if (p->num_tokens < 0) return fa::set_error(FA_ERR_INVALID_ARGUMENT, "append: num_tokens must not be negative");
+  if (p->num_tokens == 0) return 0;
+  if (p->key == nullptr || p->value == nullptr || p->k_cache == nullptr || p->v_cache == nullptr ||
+      p->k_scales == nullptr || p->v_scales == nullptr || p->slot_mapping == nullptr)
+    return fa::set_error(FA_ERR_INVALID_ARGUMENT, "append: no pointer may be NULL");
+  const int rc = check_cache8(p->dtype, p->cache_dtype, p->heads_kv, p->head_dim, p->num_blocks, p->block_size, p->k_cache,
+                              p->k_strides, p->v_cache, p->v_strides);
+  if (rc) return rc;
+  if (!rows16_ok(p->key, p->key_strides, p->num_tokens, p->heads_kv) ||
+      !rows16_ok(p->value, p->value_strides, p->num_tokens, p->heads_kv))
+    return fa::set_error(FA_ERR_UNSUPPORTED, "append: key and value need unit inner stride and rows on 16-byte boundaries");
+  return fa::launch_paged8_append(*p, static_cast<cudaStream_t>(stream));
+}
+
+int32_t fa_decode_paged8(const fa_paged8_params* p, void* stream) {
+  fa::NvtxRange r("fa_decode_paged8");
+  if (p == nullptr) return fa::set_error(FA_ERR_INVALID_ARGUMENT, "params is NULL");
+  if (p->batch <= 0 || p->heads_q <= 0 || p->max_blocks <= 0)
+    return fa::set_error(FA_ERR_INVALID_ARGUMENT, "paged batch, heads and block table width must be positive");
+  if (p->q == nullptr || p->k_cache == nullptr || p->v_cache == nullptr || p->out == nullptr || p->k_scales == nullptr ||
+      p->v_scales == nullptr || p->block_table == nullptr || p->context_lens == nullptr)
+    return fa::set_error(FA_ERR_INVALID_ARGUMENT, "q, caches, scales, block_table, context_lens and out must not be NULL");
+  int rc = check_cache8(p->dtype, p->cache_dtype, p->heads_kv, p->head_dim, p->num_blocks, p->block_size, p->k_cache,
+                        p->k_strides, p->v_cache, p->v_strides);
+  if (rc) return rc;
+  if (p->heads_q % p->heads_kv)
+    return fa::set_error(FA_ERR_INVALID_ARGUMENT, "query heads must be a multiple of cache heads");
+  if (!rows16_ok(p->q, p->q_strides, p->batch, p->heads_q) || !rows16_ok(p->out, p->o_strides, p->batch, p->heads_q))
+    return fa::set_error(FA_ERR_UNSUPPORTED, "8-bit cache: q and out need unit inner stride and rows on 16-byte boundaries");
+  const int64_t need = fa::paged8_workspace_bytes(*p);
+  if (need < 0) return (int32_t)need;
+  if (p->workspace == nullptr || p->workspace_bytes < need || reinterpret_cast<uintptr_t>(p->workspace) % 16)
+    return fa::set_error(FA_ERR_INVALID_ARGUMENT, "8-bit cache: workspace must hold %lld bytes on a 16-byte boundary",
+                         (long long)need);
+  return fa::launch_decode_paged8(*p, static_cast<cudaStream_t>(stream));
+}
+
 int64_t fa_workspace_bytes(int32_t kind, const void* params) {
   if (params == nullptr) return fa::set_error(FA_ERR_INVALID_ARGUMENT, "params is NULL");
   switch (kind) {
@@ -259,6 +347,13 @@ int64_t fa_workspace_bytes(int32_t kind, const void* params) {
       const int64_t rows = (int64_t)p->num_splits * p->batch * p->heads_q;
       return 4 * rows * (kind == FA_WS_PAGED_O_PARTIAL ? p->head_dim : 1);
     }
+  }
+  if (kind == FA_WS_PAGED8) {
+    const fa_paged8_params* p = static_cast<const fa_paged8_params*>(params);
+    if (p->batch <= 0 || p->heads_q <= 0 || p->heads_kv <= 0 || p->heads_q % p->heads_kv || p->head_dim <= 0 ||
+        p->head_dim > 256)
+      return fa::set_error(FA_ERR_INVALID_ARGUMENT, "workspace query: sizes must be positive, head_dim at most 256");
+    return fa::paged8_workspace_bytes(*p);
   }
   return fa::set_error(FA_ERR_INVALID_ARGUMENT, "unknown workspace kind %d", kind);
 }

@@ -395,6 +395,10 @@ int launch_decode_tc(const fa_decode_params& p, cudaStream_t stream);
 unsigned int* decode_ticket_words(const void* partial_buffer, int words, cudaStream_t stream);
 bool paged_tc_supported(const fa_paged_params& p);
 int launch_paged_tc(const fa_paged_params& p, cudaStream_t stream);
+int launch_paged_plan(const fa_paged_plan_params& p, cudaStream_t stream);        // fa_paged8_cache.cu
+int launch_paged8_append(const fa_paged8_append_params& p, cudaStream_t stream);
+int launch_decode_paged8(const fa_paged8_params& p, cudaStream_t stream);         // fa_paged8_decode.cu
+int64_t paged8_workspace_bytes(const fa_paged8_params& p);
 void set_decode_fault_injection(uint32_t poll_limit, int skip_tile);
 
 }  // namespace fa

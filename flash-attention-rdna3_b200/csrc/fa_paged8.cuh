@@ -1,0 +1,56 @@
+// 8-bit cache codes: conversions shared by the kernels that write the cache and the one that reads it.
+#pragma once
+
+#include "fa_common.cuh"
+
+namespace fa {
+
+// e4m3: 1 sign, 4 exponent (bias 7), 3 mantissa bits; largest finite value 448 = 1.75 * 2^8, code 0x7f is NaN.
+// int8: -127 .. 127. Every e4m3 and every int8 value is an fp16 value, so codes become fp16 without rounding.
+struct CodeE4M3 {
+  // biased fp32 exponent of 448 (minus the bias), and the fp32 mantissa field above which 2^e * 448 is too small
+  static constexpr int kTopExp = 8;
+  static constexpr uint32_t kTopMant = 0x600000u;
+  // bytes 0, 1 (lo) or 2, 3 (hi) of x as two fp16 values
+  __device__ static __forceinline__ uint32_t lo(uint32_t x) {
+    uint32_t r;
+    asm("{.reg .b16 l, h; mov.b32 {l, h}, %1; cvt.rn.f16x2.e4m3x2 %0, l;}" : "=r"(r) : "r"(x));
+    return r;
+  }
+  __device__ static __forceinline__ uint32_t hi(uint32_t x) {
+    uint32_t r;
+    asm("{.reg .b16 l, h; mov.b32 {l, h}, %1; cvt.rn.f16x2.e4m3x2 %0, h;}" : "=r"(r) : "r"(x));
+    return r;
+  }
+  // four values in units of the scale -> four codes, round to nearest even; infinities saturate, NaN stays NaN
+  __device__ static __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
+    uint32_t r;
+    asm("{.reg .b16 l, h; cvt.rn.satfinite.e4m3x2.f32 l, %2, %1; cvt.rn.satfinite.e4m3x2.f32 h, %4, %3; "
+        "mov.b32 %0, {l, h};}"
+        : "=r"(r)
+        : "f"(a), "f"(b), "f"(c), "f"(d));
+    return r;
+  }
+};
+
+struct CodeInt8 {
+  static constexpr int kTopExp = 6;  // 127 = 1.984375 * 2^6
+  static constexpr uint32_t kTopMant = 0x7e0000u;
+  // byte b ^ 0x80 = b + 128 under the exponent of 1024 is the fp16 value 1024 + 128 + b; 1152 is taken off exactly
+  __device__ static __forceinline__ uint32_t unbias(uint32_t u) {
+    const __half2 h = __hsub2(*reinterpret_cast<__half2*>(&u), __half2half2(__ushort_as_half(0x6480)));
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  __device__ static __forceinline__ uint32_t lo(uint32_t x) {
+    return unbias(__byte_perm(x ^ 0x80808080u, 0x64646464u, 0x4140));
+  }
+  __device__ static __forceinline__ uint32_t hi(uint32_t x) {
+    return unbias(__byte_perm(x ^ 0x80808080u, 0x64646464u, 0x4342));
+  }
+  __device__ static __forceinline__ int code(float v) { return max(-127, min(127, __float2int_rn(v))); }  // NaN: 0
+  __device__ static __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
+    return __byte_perm(__byte_perm(code(a), code(b), 0x0040), __byte_perm(code(c), code(d), 0x0040), 0x5410);
+  }
+};
+
+}  // namespace fa

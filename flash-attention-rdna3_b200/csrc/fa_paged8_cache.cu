@@ -1,0 +1,470 @@
+// The two operators that fill a paged 8-bit cache: page and slot planning (fa_paged_plan) and the rounding of new keys
+// and values into their pages (fa_paged8_append). include/fa_b200.h has the rules that both follow.
+#include "fa_paged8.cuh"
+
+namespace fa {
+namespace {
+
+int log2_of(int x) {
+  int s = 0;
+  while ((1 << s) < x) ++s;
+  return s;
+}
+
+// ---------------------------------------------------------------------------------------------------
+// plan
+// ---------------------------------------------------------------------------------------------------
+// Everything follows from three running sums over the requests (new tokens, pages that come back, pages needed): every
+// CTA forms them for itself in shared memory, and tokens and pages then find their request by bisection. The CTAs are
+// one cluster, whose barrier separates the reads of the lengths from the writes, so that the lengths may be updated in
+// place.
+constexpr int kPlanThreads = 512;
+constexpr int kPlanMaxCluster = 8;
+
+struct PlanArgs {
+  int batch, max_blocks, num_blocks, shift, num_tokens;
+  const int32_t* lens;
+  int64_t cl_stride;
+  const int32_t* fresh;
+  int64_t nl_stride;
+  int32_t* table;
+  int64_t bt_stride;
+  int32_t* stack;
+  const int32_t* count;
+  int64_t* slots;
+  int32_t* cu;
+  int32_t* lens_out;
+  int32_t* count_out;
+};
+
+enum : uint8_t { kUnserved = 0, kNeedsPages = 1, kEnding = 2, kNoPages = 3 };
+
+__device__ __forceinline__ int saturated(int64_t x) { return (int)min(x, (int64_t)INT32_MAX); }
+
+// Inclusive sums of two values over the CTA; *tx, *ty receive the totals. `part` holds 2 values a warp.
+__device__ __forceinline__ void block_scan2(int64_t& x, int64_t& y, int64_t* tx, int64_t* ty, int64_t (*part)[2]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t px = __shfl_up_sync(0xffffffffu, x, o), py = __shfl_up_sync(0xffffffffu, y, o);
+    if (lane >= o) {
+      x += px;
+      y += py;
+    }
+  }
+  __syncthreads();  // the last call's readers are done with `part`
+  if (lane == 31) {
+    part[warp][0] = x;
+    part[warp][1] = y;
+  }
+  __syncthreads();
+  int64_t bx = 0, by = 0, sx = 0, sy = 0;
+  for (int w = 0; w < kPlanThreads / 32; ++w) {
+    if (w < warp) {
+      bx += part[w][0];
+      by += part[w][1];
+    }
+    sx += part[w][0];
+    sy += part[w][1];
+  }
+  x += bx;
+  y += by;
+  *tx = sx;
+  *ty = sy;
+}
+
+// First index with ends[index] > value (n when there is none).
+__device__ __forceinline__ int first_above(const int* ends, int n, int value) {
+  int lo = 0, hi = n;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (ends[mid] > value) hi = mid;
+    else lo = mid + 1;
+  }
+  return lo;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanArgs a) {
+  extern __shared__ int smem[];
+  __shared__ int64_t part[kPlanThreads / 32][2];
+  int* cu_end = smem;
+  int* need_end = cu_end + a.batch;
+  int* back_end = need_end + a.batch;
+  int* len = back_end + a.batch;
+  uint8_t* state = reinterpret_cast<uint8_t*>(len + a.batch);
+  const int tid = threadIdx.x;
+  const int64_t round_up = (1 << a.shift) - 1, capacity = (int64_t)a.max_blocks << a.shift;
+  const int count = max(0, min(*a.count, a.num_blocks));
+
+  int64_t fresh_sum = 0, back_sum = 0, need_sum = 0;
+  for (int c = 0; c < a.batch; c += kPlanThreads) {
+    const int b = c + tid;
+    const bool in = b < a.batch;
+    const int64_t L = in ? a.lens[b * a.cl_stride] : 0, n = in ? a.fresh[b * a.nl_stride] : 0;
+    int64_t fresh = max(n, (int64_t)0), tf, tb;
+    int64_t back = n < 0 && L > 0 ? min((L + round_up) >> a.shift, (int64_t)a.max_blocks) : 0;
+    block_scan2(fresh, back, &tf, &tb, part);
+    const bool fits = in && n >= 0 && L >= 0 && L + n <= capacity && fresh_sum + fresh <= a.num_tokens;
+    const int64_t mine = fits ? ((L + n + round_up) >> a.shift) - ((L + round_up) >> a.shift) : 0;
+    int64_t need = mine, unused = 0, tn, tu;
+    block_scan2(need, unused, &tn, &tu, part);
+    if (in) {
+      cu_end[b] = saturated(fresh_sum + fresh);
+      back_end[b] = saturated(back_sum + back);
+      need_end[b] = saturated(need_sum + need);
+      len[b] = (int)L;
+      state[b] = n < 0 ? kEnding : !fits ? kUnserved : mine > 0 ? kNeedsPages : kNoPages;
+    }
+    fresh_sum += tf;
+    back_sum += tb;
+    need_sum += tn;
+  }
+  const int available = saturated(count + back_sum);
+  __syncthreads();
+  for (int b = tid; b < a.batch; b += kPlanThreads)
+    if (state[b] == kNeedsPages && need_end[b] > available) state[b] = kUnserved;
+  __syncthreads();
+  // every CTA has read the lengths and the count (and finished its own sums) before anyone writes
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+
+  uint32_t rank, ranks;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(ranks));
+  const int first = rank * kPlanThreads + tid, step = ranks * kPlanThreads;
+  // pages taken: the running need of the last request that is within what the stack holds
+  const int served_below = first_above(need_end, a.batch, available);
+  const int taken = served_below > 0 ? need_end[served_below - 1] : 0;
+  const int left = available - taken;
+
+  // place `p` of the stack once the pages of ending requests lie on top of it
+  auto entry = [&](int p) -> int {
+    if (p < count) return a.stack[p];
+    const int k = p - count, b = first_above(back_end, a.batch, k);
+    return a.table[(int64_t)b * a.bt_stride + (k - (b > 0 ? back_end[b - 1] : 0))];
+  };
+
+  for (int t = first; t < a.num_tokens; t += step) {
+    int64_t slot = -1;
+    const int b = first_above(cu_end, a.batch, t);
+    if (b < a.batch && (state[b] == kNeedsPages || state[b] == kNoPages)) {
+      const int pos = len[b] + (t - (b > 0 ? cu_end[b - 1] : 0));
+      const int page = pos >> a.shift, have = (int)((len[b] + round_up) >> a.shift);
+      const int id = page < have ? a.table[(int64_t)b * a.bt_stride + page]
+                                 : entry(available - 1 - (b > 0 ? need_end[b - 1] : 0) - (page - have));
+      if (id >= 0 && id < a.num_blocks) slot = ((int64_t)id << a.shift) + (pos & (int)round_up);
+    }
+    a.slots[t] = slot;
+  }
+  for (int p = first; p < taken; p += step) {
+    const int b = first_above(need_end, a.batch, p);
+    const int have = (int)((len[b] + round_up) >> a.shift);
+    a.table[(int64_t)b * a.bt_stride + have + (p - (b > 0 ? need_end[b - 1] : 0))] = entry(available - 1 - p);
+  }
+  for (int p = count + first; p < min(left, a.num_blocks); p += step) a.stack[p] = entry(p);
+  for (int b = first; b < a.batch; b += step) {
+    const int begin = b > 0 ? cu_end[b - 1] : 0;
+    a.cu[b + 1] = cu_end[b];
+    a.lens_out[b] = state[b] == kEnding ? 0 : state[b] == kUnserved ? len[b] : len[b] + (cu_end[b] - begin);
+  }
+  if (first == 0) {
+    a.cu[0] = 0;
+    *a.count_out = min(left, a.num_blocks);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------
+// append
+// ---------------------------------------------------------------------------------------------------
+// A task is the run of new tokens of one page, for one head, of keys or of values. Its rows stay in registers between
+// the maximum and the rounding (up to 8 loads of 16 bytes a lane and `warps` warps a task; longer runs are read twice).
+// A CTA holds 8 / warps tasks of the same runs: the heads of a token are neighbours in memory.
+constexpr int kAppendThreads = 256;
+constexpr int kAppendWarps = kAppendThreads / 32;
+constexpr int kAppendLoads = 8;
+
+struct AppendArgs {
+  int heads, head_dim, shift, range, warps;  // range: tokens whose runs a CTA starts; warps: warps a task
+  int64_t num_tokens, num_slots;
+  const void* src[2];
+  int64_t src_st[2], src_sh[2];
+  uint8_t* cache[2];
+  int64_t c_sb[2], c_st[2], c_sh[2];
+  float* scales[2];
+  int64_t s_sb[2], s_sh[2];
+  const int64_t* slots;
+  int64_t slot_stride;
+  int32_t* status;
+};
+
+template <typename T> struct Pair;
+template <> struct Pair<__half> { using type = __half2; };
+template <> struct Pair<__nv_bfloat16> { using type = __nv_bfloat162; };
+
+// Largest finite magnitude of eight 16-bit values, as fp32.
+template <typename T>
+__device__ __forceinline__ float finite_amax8(const uint4& v) {
+  using P = typename Pair<T>::type;
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  P m[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m[i] = __habs2(*reinterpret_cast<const P*>(&w[i]));
+  const P r = __hmax2(__hmax2(m[0], m[1]), __hmax2(m[2], m[3]));  // a NaN loses against a number
+  float best = fmaxf(DType<T>::to_float(r.x), DType<T>::to_float(r.y));
+  if (!(best < INFINITY)) {
+    best = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = DType<T>::unpack2(w[i]);
+      if (fabsf(f.x) < INFINITY) best = fmaxf(best, fabsf(f.x));
+      if (fabsf(f.y) < INFINITY) best = fmaxf(best, fabsf(f.y));
+    }
+  }
+  return best;
+}
+
+// Smallest power of two s >= 2^-126 with amax <= s * largest code.
+template <typename C8>
+__device__ __forceinline__ float scale_for(float amax) {
+  const uint32_t u = __float_as_uint(amax);
+  const int e = (int)(u >> 23) - C8::kTopExp + ((u & 0x7fffffu) > C8::kTopMant ? 1 : 0);
+  return __uint_as_float((uint32_t)max(e, 1) << 23);
+}
+
+template <typename T, typename C8>
+__global__ void __launch_bounds__(kAppendThreads) paged8_append_kernel(const AppendArgs a) {
+  __shared__ float part[2][kAppendWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int bs = 1 << a.shift;
+  const int64_t t0 = (int64_t)blockIdx.x * a.range;
+  const int task = blockIdx.y * (kAppendWarps / a.warps) + warp / a.warps, sub = warp % a.warps;
+  const bool has_task = task < 2 * a.heads;
+  const int kv = has_task ? task / a.heads : 0, head = has_task ? task % a.heads : 0;
+  const int lanes = a.head_dim / 8, rows = 32 / lanes;  // lanes a row of 16-bit values, rows a load
+  const int row = lane / lanes, col = lane % lanes;
+  const int chunk = kAppendLoads * rows * a.warps;      // tokens that the task's warps hold at once
+  const char* src = reinterpret_cast<const char*>(a.src[kv]) + (head * a.src_sh[kv] + col * 8) * 2;
+  uint8_t* cache = a.cache[kv] + head * a.c_sh[kv];
+  const int lanes8 = a.head_dim / 16, rows8 = 32 / lanes8;
+
+  // Runs that start in [t0, t0 + range): neighbours with slots in the same page. Every warp finds the same ones.
+  auto slot_at = [&](int64_t t) -> int64_t {
+    const int64_t s = t >= 0 && t < a.num_tokens ? a.slots[t * a.slot_stride] : -1;
+    return s >= 0 && s < a.num_slots ? s : -1;
+  };
+  int64_t s = slot_at(t0 + lane);
+  int64_t before = __shfl_up_sync(0xffffffffu, s, 1);
+  if (lane == 0) before = slot_at(t0 - 1);
+  const bool same = s >= 0 && before >= 0 && (s >> a.shift) == (before >> a.shift);
+  bool disorder = same && s != before + 1;
+  uint32_t starts = __ballot_sync(0xffffffffu, s >= 0 && !same && lane < a.range);
+  const uint32_t breaks = __ballot_sync(0xffffffffu, !same);
+
+  int round = 0;
+  while (starts) {
+    const int i = __ffs(starts) - 1;
+    starts &= starts - 1;
+    const int64_t slot = __shfl_sync(0xffffffffu, s, i);
+    const int64_t page = slot >> a.shift, t_first = t0 + i;
+    const int offset = (int)(slot & (bs - 1));
+    const uint32_t later = i == 31 ? 0u : breaks & (0xffffffffu << (i + 1));
+    int n;
+    if (later) {
+      n = __ffs(later) - 1 - i;
+    } else {
+      n = 32 - i;
+      for (int64_t t = t0 + 32; n < bs; t += 32) {  // the run leaves the window
+        const int64_t x = slot_at(t + lane), y = slot_at(t + lane - 1);
+        const bool cont = x >= 0 && (x >> a.shift) == page;
+        const uint32_t stop = __ballot_sync(0xffffffffu, !cont);
+        const int more = stop ? __ffs(stop) - 1 : 32;
+        if (lane < more && x != y + 1) disorder = true;
+        n += more;
+        if (stop) break;
+      }
+    }
+    n = min(n, bs - offset);
+
+    // ---- largest magnitude of the run
+    const char* first_row = src + t_first * a.src_st[kv] * 2;
+    uint4 held[kAppendLoads];
+    float amax = 0.f;
+    for (int base = 0; base < n; base += chunk) {
+#pragma unroll
+      for (int l = 0; l < kAppendLoads; ++l) {
+        const int j = base + (sub * kAppendLoads + l) * rows + row;
+        held[l] = make_uint4(0u, 0u, 0u, 0u);
+        if (has_task && row < rows && j < n)
+          held[l] = __ldg(reinterpret_cast<const uint4*>(first_row + j * a.src_st[kv] * 2));
+      }
+#pragma unroll
+      for (int l = 0; l < kAppendLoads; ++l) amax = fmaxf(amax, finite_amax8<T>(held[l]));
+    }
+    amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));
+    float* scale_at = a.scales[kv] + page * a.s_sb[kv] + head * a.s_sh[kv];
+    const float old = offset > 0 ? *scale_at : 0.f;
+    if (a.warps > 1) {
+      if (lane == 0) part[round & 1][warp] = amax;
+      __syncthreads();  // also: every warp of the task has read the old scale
+      for (int w = 0; w < a.warps; ++w) amax = fmaxf(amax, part[round & 1][warp - sub + w]);
+      ++round;
+    }
+    __syncwarp();
+    const float wanted = scale_for<C8>(amax);
+    const float scale = offset > 0 ? fmaxf(old, wanted) : wanted;
+    if (!has_task) continue;
+    if (sub == 0 && lane == 0) *scale_at = scale;
+    uint8_t* page_base = cache + page * a.c_sb[kv];
+
+    // ---- older tokens of the page, when its scale has grown
+    if (offset > 0 && scale != old) {
+      const float ratio = __fdiv_rn(old, scale);
+      const int r8 = lane / lanes8, c8 = lane % lanes8;
+      for (int j = sub * rows8 + r8; r8 < rows8 && j < offset; j += a.warps * rows8) {
+        uint4* at = reinterpret_cast<uint4*>(page_base + j * a.c_st[kv] + c8 * 16);
+        uint4 v = *at;
+        uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 lo = DType<__half>::unpack2(C8::lo(w[k])), hi = DType<__half>::unpack2(C8::hi(w[k]));
+          w[k] = C8::pack4(lo.x * ratio, lo.y * ratio, hi.x * ratio, hi.y * ratio);
+        }
+        *at = v;
+      }
+    }
+
+    // ---- the new tokens. Dividing by a power of two is multiplying by its inverse; a scale that the caller made and
+    // that is none is divided by.
+    const bool exact_inverse = (__float_as_uint(scale) & 0x7fffffu) == 0;
+    const float inverse = __fdiv_rn(1.f, scale);
+    for (int base = 0; base < n; base += chunk) {
+#pragma unroll
+      for (int l = 0; l < kAppendLoads; ++l) {
+        const int j = base + (sub * kAppendLoads + l) * rows + row;
+        if (row >= rows || j >= n) continue;
+        uint4 v = held[l];
+        if (n > chunk) v = __ldg(reinterpret_cast<const uint4*>(first_row + j * a.src_st[kv] * 2));
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        float f[8];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 p = DType<T>::unpack2(w[k]);
+          f[2 * k] = p.x * inverse;
+          f[2 * k + 1] = p.y * inverse;
+          if (!exact_inverse) {
+            f[2 * k] = __fdiv_rn(p.x, scale);
+            f[2 * k + 1] = __fdiv_rn(p.y, scale);
+          }
+        }
+        *reinterpret_cast<uint2*>(page_base + (offset + j) * a.c_st[kv] + col * 8) =
+            make_uint2(C8::pack4(f[0], f[1], f[2], f[3]), C8::pack4(f[4], f[5], f[6], f[7]));
+      }
+    }
+  }
+  if (disorder && a.status != nullptr) *a.status = FA_STATUS_SLOT_ORDER;
+}
+
+int check_launch(const char* what, cudaError_t e) {
+  if (e == cudaSuccess) e = cudaGetLastError();
+  else cudaGetLastError();
+  return e == cudaSuccess ? 0 : set_error(FA_ERR_LAUNCH, "%s launch failed: %s", what, cudaGetErrorString(e));
+}
+
+}  // namespace
+
+int launch_paged_plan(const fa_paged_plan_params& p, cudaStream_t stream) {
+  if (p.num_tokens > INT32_MAX || ((int64_t)p.max_blocks * p.block_size) > INT32_MAX)
+    return set_error(FA_ERR_UNSUPPORTED, "plan: more than 2^31 - 1 tokens");
+  PlanArgs a = {};
+  a.batch = p.batch;
+  a.max_blocks = p.max_blocks;
+  a.num_blocks = p.num_blocks;
+  a.shift = log2_of(p.block_size);
+  a.num_tokens = (int)p.num_tokens;
+  a.lens = p.context_lens;
+  a.cl_stride = p.cl_stride;
+  a.fresh = p.new_lens;
+  a.nl_stride = p.nl_stride;
+  a.table = p.block_table;
+  a.bt_stride = p.bt_stride;
+  a.stack = p.free_blocks;
+  a.count = p.free_count;
+  a.slots = p.slot_mapping;
+  a.cu = p.cu_seqlens;
+  a.lens_out = p.context_lens_out;
+  a.count_out = p.free_count_out;
+  const int smem = p.batch * 17;
+  if (smem > 40 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) {
+      cudaGetLastError();
+      return set_error(FA_ERR_LAUNCH, "plan: cannot get %d bytes of shared memory: %s", smem, cudaGetErrorString(e));
+    }
+  }
+  const int64_t work = p.num_tokens > p.batch ? p.num_tokens : p.batch;
+  int cluster = 1;
+  while (cluster < kPlanMaxCluster && cluster * 2 * kPlanThreads <= work) cluster *= 2;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = cluster;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(cluster);
+  cfg.blockDim = dim3(kPlanThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return check_launch("plan", cudaLaunchKernelEx(&cfg, paged_plan_kernel, a));
+}
+
+int launch_paged8_append(const fa_paged8_append_params& p, cudaStream_t stream) {
+  AppendArgs a = {};
+  a.heads = p.heads_kv;
+  a.head_dim = p.head_dim;
+  a.shift = log2_of(p.block_size);
+  a.num_tokens = p.num_tokens;
+  a.num_slots = (int64_t)p.num_blocks * p.block_size;
+  a.src[0] = p.key;
+  a.src[1] = p.value;
+  a.src_st[0] = p.key_strides[0];
+  a.src_sh[0] = p.key_strides[1];
+  a.src_st[1] = p.value_strides[0];
+  a.src_sh[1] = p.value_strides[1];
+  a.cache[0] = static_cast<uint8_t*>(p.k_cache);
+  a.cache[1] = static_cast<uint8_t*>(p.v_cache);
+  for (int kv = 0; kv < 2; ++kv) {
+    const int64_t* st = kv ? p.v_strides : p.k_strides;
+    const int64_t* ss = kv ? p.vs_strides : p.ks_strides;
+    a.c_sb[kv] = st[0];
+    a.c_st[kv] = st[1];
+    a.c_sh[kv] = st[2];
+    a.scales[kv] = kv ? p.v_scales : p.k_scales;
+    a.s_sb[kv] = ss[0];
+    a.s_sh[kv] = ss[1];
+  }
+  a.slots = p.slot_mapping;
+  a.slot_stride = p.slot_stride;
+  a.status = p.status;
+  const int rows = 32 / (p.head_dim / 8);
+  a.warps = 1;
+  while (a.warps < kAppendWarps && a.warps * kAppendLoads * rows < p.block_size) a.warps *= 2;
+  const int64_t tasks = (2 * p.heads_kv + kAppendWarps / a.warps - 1) / (kAppendWarps / a.warps);
+  if (tasks > 65535) return set_error(FA_ERR_UNSUPPORTED, "append: too many heads");
+  // a CTA starts the runs of `range` tokens: one while the grid is small, up to a page's (at most 32) for prompts
+  a.range = 1;
+  while (a.range < 32 && a.range < p.block_size && p.num_tokens * tasks / (2 * a.range) >= 1184) a.range *= 2;
+  const int64_t grid = (p.num_tokens + a.range - 1) / a.range;
+  if (grid > INT32_MAX) return set_error(FA_ERR_UNSUPPORTED, "append: too many tokens");
+  const dim3 g((unsigned)grid, (unsigned)tasks);
+  const bool e4m3 = p.cache_dtype == FA_CACHE_E4M3;
+  if (p.dtype == FA_F16) {
+    if (e4m3) paged8_append_kernel<__half, CodeE4M3><<<g, kAppendThreads, 0, stream>>>(a);
+    else paged8_append_kernel<__half, CodeInt8><<<g, kAppendThreads, 0, stream>>>(a);
+  } else {
+    if (e4m3) paged8_append_kernel<__nv_bfloat16, CodeE4M3><<<g, kAppendThreads, 0, stream>>>(a);
+    else paged8_append_kernel<__nv_bfloat16, CodeInt8><<<g, kAppendThreads, 0, stream>>>(a);
+  }
+  return check_launch("append", cudaSuccess);
+}
+
+}  // namespace fa

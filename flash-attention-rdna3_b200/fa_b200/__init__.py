@@ -11,6 +11,12 @@ from .interface import (
     flash_attn_func,
     flash_attn_varlen_func,
 )
+from .paged_cache import (
+    PagedKVCache8,
+    flash_attention_decode_paged_8bit,
+    paged_kv_append,
+    paged_kv_plan,
+)
 from .sdpa import (
     disable_flash_attention,
     disable_rdna3_flash_attention,
@@ -27,6 +33,10 @@ __all__ = [
     "flash_attention_decode",
     "flash_attention_varlen",
     "flash_attention_decode_paged",
+    "flash_attention_decode_paged_8bit",
+    "paged_kv_append",
+    "paged_kv_plan",
+    "PagedKVCache8",
     "flash_attn_func",
     "flash_attn_varlen_func",
     "alibi_slopes",

@@ -16,6 +16,10 @@ FA_BWD_DELTA, FA_BWD_DKDV, FA_BWD_DQ = 1, 2, 4
 FA_WS_BWD_DELTA, FA_WS_DECODE_O_PARTIAL, FA_WS_DECODE_LSE_PARTIAL, FA_WS_PAGED_O_PARTIAL, FA_WS_PAGED_LSE_PARTIAL = 1, 2, 3, 4, 5
 FA_WS_BWD_DS = 6
 FA_WS_FWD_P = 7
+FA_WS_PAGED8 = 8
+FA_CACHE_E4M3, FA_CACHE_INT8 = 0, 1
+FA_PLAN_MAX_BATCH = 8192
+FA_STATUS_SLOT_ORDER = 101
 ABI_VERSION = 3
 
 I64x4 = C.c_int64 * 4
@@ -123,6 +127,53 @@ class TinyParams(C.Structure):
     ]
 
 
+class PagedPlanParams(C.Structure):
+    _fields_ = [
+        ("batch", C.c_int32), ("max_blocks", C.c_int32), ("num_blocks", C.c_int32), ("block_size", C.c_int32),
+        ("num_tokens", C.c_int64),
+        ("context_lens", C.c_void_p), ("cl_stride", C.c_int64),
+        ("new_lens", C.c_void_p), ("nl_stride", C.c_int64),
+        ("block_table", C.c_void_p), ("bt_stride", C.c_int64),
+        ("free_blocks", C.c_void_p), ("free_count", C.c_void_p),
+        ("slot_mapping", C.c_void_p), ("cu_seqlens", C.c_void_p),
+        ("context_lens_out", C.c_void_p), ("free_count_out", C.c_void_p),
+    ]
+
+
+class Paged8AppendParams(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("cache_dtype", C.c_int32),
+        ("heads_kv", C.c_int32), ("head_dim", C.c_int32), ("num_blocks", C.c_int32), ("block_size", C.c_int32),
+        ("num_tokens", C.c_int64),
+        ("key", C.c_void_p), ("key_strides", I64x3),
+        ("value", C.c_void_p), ("value_strides", I64x3),
+        ("k_cache", C.c_void_p), ("k_strides", I64x4),
+        ("v_cache", C.c_void_p), ("v_strides", I64x4),
+        ("k_scales", C.c_void_p), ("ks_strides", I64x2),
+        ("v_scales", C.c_void_p), ("vs_strides", I64x2),
+        ("slot_mapping", C.c_void_p), ("slot_stride", C.c_int64),
+        ("status", C.c_void_p),
+    ]
+
+
+class Paged8Params(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("cache_dtype", C.c_int32),
+        ("batch", C.c_int32), ("heads_q", C.c_int32), ("heads_kv", C.c_int32), ("head_dim", C.c_int32),
+        ("num_blocks", C.c_int32), ("block_size", C.c_int32), ("max_blocks", C.c_int32),
+        ("q", C.c_void_p), ("q_strides", I64x3),
+        ("k_cache", C.c_void_p), ("k_strides", I64x4),
+        ("v_cache", C.c_void_p), ("v_strides", I64x4),
+        ("k_scales", C.c_void_p), ("ks_strides", I64x2),
+        ("v_scales", C.c_void_p), ("vs_strides", I64x2),
+        ("block_table", C.c_void_p), ("bt_strides", I64x2),
+        ("context_lens", C.c_void_p), ("cl_stride", C.c_int64),
+        ("out", C.c_void_p), ("o_strides", I64x3),
+        ("softmax_scale", C.c_float),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
+    ]
+
+
 # name -> (restype, argtypes); the symbol list that include/fa_b200.h declares
 SYMBOLS = {
     "fa_abi_version": (C.c_int32, []),
@@ -138,6 +189,9 @@ SYMBOLS = {
     "fa_decode_splitk_noalloc": (C.c_int32, [C.POINTER(DecodeParams), C.c_void_p]),
     "fa_combine": (C.c_int32, [C.POINTER(CombineParams), C.c_void_p]),
     "fa_decode_paged": (C.c_int32, [C.POINTER(PagedParams), C.c_void_p]),
+    "fa_paged_plan": (C.c_int32, [C.POINTER(PagedPlanParams), C.c_void_p]),
+    "fa_paged8_append": (C.c_int32, [C.POINTER(Paged8AppendParams), C.c_void_p]),
+    "fa_decode_paged8": (C.c_int32, [C.POINTER(Paged8Params), C.c_void_p]),
     "fa_tiny_fwd": (C.c_int32, [C.POINTER(TinyParams), C.c_void_p]),
     "fa_workspace_bytes": (C.c_int64, [C.c_int32, C.c_void_p]),
     "fa_test_decode_fault": (None, [C.c_uint32, C.c_int32]),

@@ -233,3 +233,131 @@ def validate_paged_inputs(query, key, value, block_table, context_lens):
     if block_table.shape[1] <= 0:
         raise ValueError("block_table must contain at least one logical block")
     _require_platform(query.device)
+
+
+# ---------------------------------------------------------------------------------------------------
+# paged 8-bit KV cache
+# ---------------------------------------------------------------------------------------------------
+CACHE8_DTYPES = (torch.float8_e4m3fn, torch.int8)
+CACHE8_HEAD_DIMS = (16, 32, 64, 128, 256)
+PLAN_MAX_BATCH = 8192
+
+
+def _validate_cache8(k_cache, v_cache, k_scales, v_scales):
+    """Contracts of the caches (blocks, block, heads, dim) and their scales (blocks, heads)."""
+    for name, cache in (("k_cache", k_cache), ("v_cache", v_cache)):
+        _require_tensor(name, cache)
+        if cache.dim() != 4:
+            raise ValueError("8-bit caches must be (blocks, block, heads, dim)")
+        if cache.dtype not in CACHE8_DTYPES:
+            raise ValueError("8-bit caches must be float8_e4m3fn or int8")
+    shape = k_cache.shape
+    if shape != v_cache.shape or k_cache.dtype != v_cache.dtype:
+        raise ValueError("8-bit key and value caches must have the same shape and dtype")
+    blocks, block_size, heads, dim = shape
+    if min(blocks, block_size, heads, dim) <= 0:
+        raise ValueError("8-bit cache blocks, block size, heads and head_dim must be positive")
+    if block_size & (block_size - 1):
+        raise ValueError("paged cache block size must be a power of two")
+    if dim not in CACHE8_HEAD_DIMS:
+        raise ValueError(f"head_dim {dim} not supported by 8-bit caches; expected one of {CACHE8_HEAD_DIMS}")
+    for name, cache in (("k_cache", k_cache), ("v_cache", v_cache)):
+        st = cache.stride()
+        # (the library refuses a base address off a 16-byte boundary: a traced tensor has none to look at)
+        if st[3] != 1 or any(n > 1 and (s <= 0 or s % 16) for n, s in zip(shape[:3], st[:3])):
+            raise ValueError(f"{name} must have unit inner stride, no broadcast dimension and rows aligned to 16 bytes")
+    for name, scales in (("k_scales", k_scales), ("v_scales", v_scales)):
+        _require_tensor(name, scales)
+        if scales.dtype != torch.float32 or scales.shape != (blocks, heads):
+            raise ValueError(f"{name} must be float32 of shape (blocks, heads) = ({blocks}, {heads})")
+    device = k_cache.device
+    if not (v_cache.device == k_scales.device == v_scales.device == device):
+        raise ValueError("8-bit caches and scales must be on the same device")
+
+
+def validate_paged8_inputs(query, k_cache, v_cache, k_scales, v_scales, block_table, context_lens):
+    """Contracts of decode over the 8-bit cache."""
+    _validate_cache8(k_cache, v_cache, k_scales, v_scales)
+    _require_tensor("query", query)
+    if query.dim() != 3:
+        raise ValueError("paged query must be (batch, heads, dim)")
+    if query.dtype not in LOW_PRECISION_DTYPES:
+        raise ValueError("paged query must be float16 or bfloat16")
+    batch, heads, dim = query.shape
+    if min(batch, heads) <= 0:
+        raise ValueError("paged batch and heads must be positive")
+    if dim != k_cache.shape[3]:
+        raise ValueError("paged query and cache head_dim must match")
+    if heads % k_cache.shape[2]:
+        raise ValueError("query heads must be a multiple of cache heads")
+    device = query.device
+    if k_cache.device != device:
+        raise ValueError("paged query and caches must be on the same device")
+    for name, meta, ndim in (("block_table", block_table, 2), ("context_lens", context_lens, 1)):
+        _require_tensor(name, meta)
+        if meta.device != device or meta.dtype != torch.int32:
+            raise ValueError(f"{name} must be an int32 tensor on {device}")
+        if meta.dim() != ndim or meta.shape[0] != batch:
+            raise ValueError(f"{name} has an invalid shape for batch size {batch}")
+    if block_table.shape[1] <= 0:
+        raise ValueError("block_table must contain at least one logical block")
+    _require_platform(device)
+
+
+def validate_paged8_append_inputs(key, value, k_cache, v_cache, k_scales, v_scales, slot_mapping):
+    """Contracts of the rounding of new keys and values into the 8-bit cache."""
+    _validate_cache8(k_cache, v_cache, k_scales, v_scales)
+    for name, scales in (("k_scales", k_scales), ("v_scales", v_scales)):
+        if any(n > 1 and s <= 0 for n, s in zip(scales.shape, scales.stride())):
+            raise ValueError(f"{name} must have no broadcast dimension")
+    _require_tensor("key", key)
+    _require_tensor("value", value)
+    if key.dim() != 3 or key.shape != value.shape:
+        raise ValueError("key and value must have the same shape (tokens, heads, dim)")
+    if key.dtype not in LOW_PRECISION_DTYPES or key.dtype != value.dtype:
+        raise ValueError("key and value must share a float16 or bfloat16 dtype")
+    if key.shape[1:] != k_cache.shape[2:]:
+        raise ValueError("key and cache must have the same heads and head_dim")
+    _require_tensor("slot_mapping", slot_mapping)
+    device = key.device
+    if not (value.device == k_cache.device == device):
+        raise ValueError("key, value and caches must be on the same device")
+    if slot_mapping.device != device or slot_mapping.dtype != torch.int64:
+        raise ValueError(f"slot_mapping must be an int64 tensor on {device}")
+    if slot_mapping.shape != (key.shape[0],):
+        raise ValueError("slot_mapping must have one entry for each token")
+    _require_platform(device)
+
+
+def validate_paged_plan_inputs(context_lens, new_lens, block_table, free_blocks, free_count, num_tokens, block_size,
+                               inplace=False):
+    """Contracts of page planning."""
+    for name, t, ndim in (("context_lens", context_lens, 1), ("new_lens", new_lens, 1), ("block_table", block_table, 2),
+                          ("free_blocks", free_blocks, 1), ("free_count", free_count, 1)):
+        _require_tensor(name, t)
+        if t.dtype != torch.int32 or t.device != context_lens.device:
+            raise ValueError(f"{name} must be an int32 tensor on {context_lens.device}")
+        if t.dim() != ndim:
+            raise ValueError(f"{name} must have {ndim} dimension{'s' if ndim > 1 else ''}")
+    batch = context_lens.shape[0]
+    if new_lens.shape[0] != batch or block_table.shape[0] != batch:
+        raise ValueError("context_lens, new_lens and block_table must describe the same batch size")
+    if not 0 < batch <= PLAN_MAX_BATCH:
+        raise ValueError(f"plan takes 1 to {PLAN_MAX_BATCH} requests")
+    if block_table.shape[1] <= 0 or free_blocks.shape[0] <= 0:
+        raise ValueError("block_table must contain at least one logical block and free_blocks one page")
+    if block_table.stride(1) != 1 or (batch > 1 and block_table.stride(0) < block_table.shape[1]):
+        raise ValueError("block_table must have unit inner stride and rows that do not overlap")
+    if free_blocks.stride(0) != 1:
+        raise ValueError("free_blocks must be contiguous")
+    if free_count.shape[0] != 1:
+        raise ValueError("free_count must have one element")
+    if inplace and batch > 1 and context_lens.stride(0) != 1:
+        raise ValueError("context_lens must be contiguous to be updated in place")
+    if not _is_plain_int(num_tokens) or not 0 <= num_tokens < 2 ** 31:
+        raise ValueError("num_tokens must be a nonnegative integer below 2^31")
+    if not _is_plain_int(block_size) or block_size <= 0 or block_size & (block_size - 1):
+        raise ValueError("paged cache block size must be a power of two")
+    if block_table.shape[1] * block_size >= 2 ** 31:
+        raise ValueError("block_table must span fewer than 2^31 tokens")
+    _require_platform(context_lens.device)

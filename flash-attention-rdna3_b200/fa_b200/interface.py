@@ -191,7 +191,8 @@ def _status_word(device):
 
 
 def check_status(device=None):
-    """Synchronise and raise if any kernel on `device` reported a lost wait since the last check."""
+    """Synchronise and raise if any kernel on `device` reported a lost wait (or `paged_kv_append` a slot mapping that it
+    cannot follow) since the last check."""
     index = torch.cuda.current_device() if device is None else torch.device(device).index
     word = _status_words.get(index)
     if word is None:
@@ -199,6 +200,8 @@ def check_status(device=None):
     code = int(word.item())
     if code != 0:
         word.zero_()
+        if code == _lib.FA_STATUS_SLOT_ORDER:
+            raise RuntimeError("paged_kv_append: the slots of a page repeat or do not rise by one in slot_mapping")
         raise RuntimeError(f"fa_b200 kernel reported an internal wait timeout (code {code})")
 
 

@@ -222,6 +222,83 @@ typedef struct fa_paged_params {
                                batch may be at most 256 and at most the SM count. */
 } fa_paged_params;
 
+/* ---- paged KV cache held in 8 bits (no counterpart in the reference, whose caches are 16-bit and filled by the caller) ----
+
+   Caches (num_blocks, block_size, heads_kv, head_dim) of fa_cache_dtype with unit inner stride, rows on 16-byte
+   boundaries and head_dim a multiple of 16 up to 256; block_size a power of two. One fp32 scale for each block and kv
+   head, (num_blocks, heads_kv): a stored code c stands for c * scale. The three entry points below are what a server
+   runs in every step: fa_paged_plan once, then fa_paged8_append and fa_decode_paged8 in every layer. */
+enum fa_cache_dtype { FA_CACHE_E4M3 = 0, FA_CACHE_INT8 = 1 };
+
+/* Pages and slots for the tokens of one step. Request b holds context_lens[b] tokens and brings new_lens[b] more
+   (packed one request after the other: cu_seqlens, written here, has their offsets); new_lens[b] < 0 ends it.
+     1. The pages of ending requests go on top of the stack free_blocks[0 .. free_count), request by request.
+     2. Request b needs ceil((L + n) / bs) - ceil(L / bs) new pages. It is served when L >= 0, its tokens fit into the
+        block table's row and into num_tokens, and the pages needed up to and including it (of the requests that fit)
+        do not exceed the stack. Served requests pop their pages from the top in the order of the requests.
+     3. slot_mapping[t] = page * block_size + offset of every new token; -1 for the tokens of requests that are not
+        served and behind the last token. The block table gets the new pages; entries past them stay as they were.
+     4. context_lens_out = L + n (served), 0 (ended), L (not served); free_count_out = what the stack holds after it.
+   context_lens_out and free_count_out may be the inputs themselves. Where they are not, a second call with the same
+   inputs gives the same results. Page ids outside [0, num_blocks) give slot -1. */
+typedef struct fa_paged_plan_params {
+  int32_t batch, max_blocks, num_blocks, block_size;
+  int64_t num_tokens;             /* entries of slot_mapping */
+  const int32_t* context_lens; int64_t cl_stride;
+  const int32_t* new_lens; int64_t nl_stride;
+  int32_t* block_table; int64_t bt_stride;  /* (batch, max_blocks), unit inner stride; read and written */
+  int32_t* free_blocks;           /* (num_blocks,), read and written */
+  const int32_t* free_count;      /* one value */
+  int64_t* slot_mapping;          /* (num_tokens,) */
+  int32_t* cu_seqlens;            /* (batch + 1,) */
+  int32_t* context_lens_out;      /* (batch,) */
+  int32_t* free_count_out;        /* one value */
+} fa_paged_plan_params;
+#define FA_PLAN_MAX_BATCH 8192
+
+/* Rounds new keys and values (num_tokens, heads_kv, head_dim; fp16 or bf16) to 8 bits at their slots. Scales are powers
+   of two: the smallest s >= 2^-126 with |x| <= s * largest code (448 or 127) over the finite values that a page and
+   head receive. Codes are round-to-nearest-even of x / s; infinities become the largest code, NaN stays NaN (int8: 0).
+   A page whose first new token is not its first slot keeps the tokens in front of it: its scale becomes
+   max(old, s), and where that grows the old codes are rounded again to the new scale.
+   The new tokens of a page are neighbours in slot_mapping with rising slots, as fa_paged_plan leaves them; a page whose
+   slots repeat or fall sets *status to FA_STATUS_SLOT_ORDER (its content is then unspecified). Slots outside
+   [0, num_blocks * block_size) are skipped. */
+typedef struct fa_paged8_append_params {
+  int32_t dtype, cache_dtype;
+  int32_t heads_kv, head_dim, num_blocks, block_size;
+  int64_t num_tokens;
+  const void* key;   int64_t key_strides[3];
+  const void* value; int64_t value_strides[3];
+  void* k_cache; int64_t k_strides[4];
+  void* v_cache; int64_t v_strides[4];
+  float* k_scales; int64_t ks_strides[2];
+  float* v_scales; int64_t vs_strides[2];
+  const int64_t* slot_mapping; int64_t slot_stride;
+  int32_t* status;                /* may be NULL */
+} fa_paged8_append_params;
+#define FA_STATUS_SLOT_ORDER 101
+
+/* Decode attention over the 8-bit cache: q, out (batch, heads_q, head_dim) fp16 or bf16, the rest as in
+   fa_paged_params (context lengths are clamped to the table, page ids out of range contribute nothing, an empty context
+   gives zeros). workspace: fa_workspace_bytes(FA_WS_PAGED8, p) bytes, aligned to 16; it depends on the current device's
+   SM count and on the head layout, not on the contexts. */
+typedef struct fa_paged8_params {
+  int32_t dtype, cache_dtype;
+  int32_t batch, heads_q, heads_kv, head_dim;
+  int32_t num_blocks, block_size, max_blocks;
+  const void* q; int64_t q_strides[3];
+  const void* k_cache; int64_t k_strides[4];
+  const void* v_cache; int64_t v_strides[4];
+  const float* k_scales; int64_t ks_strides[2];
+  const float* v_scales; int64_t vs_strides[2];
+  const int32_t* block_table; int64_t bt_strides[2];
+  const int32_t* context_lens; int64_t cl_stride;
+  void* out; int64_t o_strides[3];
+  float softmax_scale;
+  void* workspace; int64_t workspace_bytes;
+} fa_paged8_params;
+
 /* FP32 short-sequence attention: q, k, v, out (batch, heads, seqlen <= 32, 128), optional bias. */
 typedef struct fa_tiny_params {
   int32_t batch, heads, seqlen, head_dim;
@@ -252,7 +329,8 @@ enum fa_workspace_kind {
   FA_WS_PAGED_O_PARTIAL = 4,    /* fa_paged_params  -> o_partial */
   FA_WS_PAGED_LSE_PARTIAL = 5,  /* fa_paged_params  -> lse_partial */
   FA_WS_BWD_DS = 6,             /* fa_attn_params   -> ds_workspace of fa_bwd (optional; 0 when the problem cannot use one) */
-  FA_WS_FWD_P = 7               /* fa_attn_params   -> ds_workspace of fa_fwd (16-bit head dims above 256, fp32 to 256; else 0) */
+  FA_WS_FWD_P = 7,              /* fa_attn_params   -> ds_workspace of fa_fwd (16-bit head dims above 256, fp32 to 256; else 0) */
+  FA_WS_PAGED8 = 8              /* fa_paged8_params -> workspace of fa_decode_paged8 */
 };
 FA_API int64_t fa_workspace_bytes(int32_t kind, const void* params);
 
@@ -303,6 +381,11 @@ FA_API int32_t fa_enable_peer_access(int32_t peer_device);
 /* Paged-KV decode. Replaces the _attention_decode_paged (+ combine) launches,
    fa_rdna3/interface.py:703-727 (kernel fa_rdna3/kernels/paged.py:17-89). */
 FA_API int32_t fa_decode_paged(const fa_paged_params* p, void* stream);
+
+/* See fa_paged_plan_params, fa_paged8_append_params and fa_paged8_params. */
+FA_API int32_t fa_paged_plan(const fa_paged_plan_params* p, void* stream);
+FA_API int32_t fa_paged8_append(const fa_paged8_append_params* p, void* stream);
+FA_API int32_t fa_decode_paged8(const fa_paged8_params* p, void* stream);
 
 /* Test hook, no counterpart in the reference: makes the NEXT tensor-core decode launch (dense or paged) of the
    calling thread use `poll_limit` polls per barrier wait (0 = the default, about a second) and leave out the

@@ -1,0 +1,592 @@
+"""The paged 8-bit KV cache on the GPU: planning, appending and decoding against the oracle, and the three together."""
+import pytest
+import torch
+
+import fa_b200
+from fa_b200 import paged_cache
+from oracle import paged_cache_oracle as oracle
+
+pytestmark = pytest.mark.gpu
+E4M3 = torch.float8_e4m3fn
+CACHES = [E4M3, torch.int8]
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def ints(values, device="cuda"):
+    return torch.tensor(values, dtype=torch.int32, device=device)
+
+
+def bytes_equal(a, b):
+    return torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+# ---------------------------------------------------------------------------------------------------
+# plan
+# ---------------------------------------------------------------------------------------------------
+def random_plan(seed, batch, bs, width, max_new, spare, ends=0.2, pad=3):
+    g = gen(seed)
+    cap = width * bs
+    lens = [int(x) for x in torch.randint(0, cap + 1, (batch,), generator=g)]
+    new = [int(x) for x in torch.randint(0, max_new + 1, (batch,), generator=g)]
+    new = [-int(e) if e else n for n, e in zip(new, (torch.rand(batch, generator=g) < ends).int())]
+    held = [-(-n // bs) for n in lens]
+    blocks = sum(held) + spare
+    ids = torch.randperm(blocks, generator=g).tolist()
+    table = torch.full((batch, width), -1, dtype=torch.int32)
+    for b, n in enumerate(held):
+        for j in range(n):
+            table[b, j] = ids.pop()
+    stack = torch.full((blocks,), -1, dtype=torch.int32)
+    stack[:len(ids)] = ints(ids, "cpu")
+    return ints(lens), ints(new), table.cuda(), stack.cuda(), ints([len(ids)]), sum(max(n, 0) for n in new) + pad
+
+
+def check_plan(args, bs, inplace=False):
+    lens, new, table, stack, count, tokens = args
+    want = oracle.plan_ref(lens.tolist(), new.tolist(), table.cpu(), stack.cpu(), int(count), tokens, bs)
+    before = lens.clone(), count.clone()
+    got = fa_b200.paged_kv_plan(lens, new, table, stack, count, tokens, bs, inplace=inplace)
+    for name, a, b in zip(("slots", "cu", "lens", "count", "table", "stack"),
+                          (got[0], got[1], got[2], got[3][0], table, stack), want):
+        assert a.tolist() == b, name
+    if inplace:
+        assert got[2] is lens and got[3] is count
+    else:
+        assert torch.equal(lens, before[0]) and torch.equal(count, before[1])
+    return got
+
+
+@pytest.mark.parametrize("batch, bs, width, max_new, spare", [
+    (1, 16, 4, 1, 2), (3, 1, 9, 4, 20), (17, 16, 12, 40, 60), (64, 16, 128, 1, 9), (33, 64, 8, 300, 200),
+    (512, 8, 30, 9, 500), (513, 16, 20, 30, 1000), (1500, 32, 6, 20, 1500), (40, 256, 3, 700, 100)])
+@pytest.mark.parametrize("inplace", [False, True])
+def test_plan(batch, bs, width, max_new, spare, inplace):
+    check_plan(random_plan(batch + bs, batch, bs, width, max_new, spare), bs, inplace)
+
+
+def test_plan_is_repeatable_with_lengths_kept():
+    args = random_plan(5, 50, 16, 20, 60, 90)
+    first = check_plan(args, 16)
+    table, stack = args[2].clone(), args[3].clone()
+    second = fa_b200.paged_kv_plan(*args, 16)
+    assert all(torch.equal(a, b) for a, b in zip(first, second))
+    assert torch.equal(table, args[2]) and torch.equal(stack, args[3])
+
+
+def test_plan_when_pages_run_out_and_rows_are_full():
+    for spare in (0, 1, 5, 17):
+        check_plan(random_plan(spare, 40, 16, 10, 70, spare, ends=0.05), 16)
+
+
+def test_plan_with_fewer_slots_than_tokens():
+    lens, new, table, stack, count, tokens = random_plan(3, 30, 16, 20, 50, 200)
+    for n in (0, 1, tokens // 2):
+        check_plan((lens, new, table.clone(), stack.clone(), count, n), 16)
+
+
+def test_plan_everything_ends_and_nothing_is_there():
+    args = random_plan(8, 20, 16, 6, 5, 3)
+    check_plan((args[0], torch.full_like(args[1], -1), *args[2:5], 4), 16)
+    check_plan((torch.zeros_like(args[0]), torch.zeros_like(args[1]), torch.full_like(args[2], -1), args[3],
+                ints([0]), 0), 16)
+
+
+def test_plan_strange_values():
+    """Negative and too large lengths, ids outside the pool, a count outside the stack: no slot, nothing written outside."""
+    lens, new, table, stack, count, tokens = random_plan(11, 12, 16, 8, 40, 60, ends=0.0)
+    lens[3], lens[5] = -7, 10 ** 9
+    stack[:] = torch.where(torch.arange(stack.numel(), device="cuda") % 3 == 0, stack + 10 ** 6, stack)
+    check_plan((lens, new, table, stack, count, tokens), 16)
+    lens, new, table, stack, count, tokens = random_plan(12, 12, 16, 8, 40, 60, ends=0.3)
+    fa_b200.paged_kv_plan(lens, new, table, stack, ints([10 ** 9]), tokens, 16)
+    fa_b200.paged_kv_plan(lens, new, table, stack, ints([-5]), tokens, 16)
+    torch.cuda.synchronize()
+
+
+def test_plan_strided_inputs():
+    lens, new, table, stack, count, tokens = random_plan(21, 25, 16, 9, 30, 60)
+    wide = torch.full((25, 31), -9, dtype=torch.int32, device="cuda")
+    wide[:, 4:13] = table
+    lens2, new2 = torch.stack((lens, lens), 1)[:, 0], torch.stack((new, new, new), 1)[:, 1]
+    check_plan((lens2, new2, wide[:, 4:13], stack, count, tokens), 16)
+    assert (wide[:, :4] == -9).all() and (wide[:, 13:] == -9).all()
+
+
+# ---------------------------------------------------------------------------------------------------
+# append
+# ---------------------------------------------------------------------------------------------------
+def filled_cache(seed, blocks, bs, heads, dim, dtype):
+    """Codes over the whole range under scales of different size (what lies in pages before a step)."""
+    g = gen(seed)
+    x = torch.randn(blocks, bs, heads, dim, generator=g)
+    scales = torch.exp2(torch.randint(-6, 2, (blocks, heads), generator=g).float())
+    if dtype == torch.int8:
+        codes = (x * 40).round().clamp(-127, 127).to(torch.int8)
+    else:
+        codes = (x * 60).clamp(-448, 448).to(E4M3)
+    return codes.cuda(), scales.cuda()
+
+
+def runs_to_slots(runs, bs):
+    """runs: (page, first offset, tokens); page None: tokens without a slot."""
+    slots = []
+    for page, o, n in runs:
+        slots += [-1] * n if page is None else [page * bs + o + i for i in range(n)]
+    return torch.tensor(slots, dtype=torch.int64, device="cuda")
+
+
+def random_runs(seed, blocks, bs, requests, longest):
+    """Requests whose first page may be half full, over a random permutation of pages."""
+    g = gen(seed)
+    pages = torch.randperm(blocks, generator=g).tolist()
+    runs = []
+    for _ in range(requests):
+        o, n = int(torch.randint(0, bs, (1,), generator=g)), int(torch.randint(1, longest + 1, (1,), generator=g))
+        while n > 0 and pages:
+            m = min(n, bs - o)
+            runs.append((pages.pop(), o, m))
+            n, o = n - m, 0
+        if int(torch.randint(0, 4, (1,), generator=g)) == 0:
+            runs.append((None, 0, 2))
+    return runs
+
+
+def check_append(key, value, k, v, ks, vs, slots):
+    want = [oracle.append_ref(x, c, s, slots.tolist()) for x, c, s in ((key, k, ks), (value, v, vs))]
+    fa_b200.paged_kv_append(key, value, k, v, ks, vs, slots)
+    for c, s, (codes, scales) in ((k, ks, want[0]), (v, vs, want[1])):
+        assert torch.equal(s.double(), scales)
+        assert torch.equal(torch.nan_to_num(c.double(), nan=1e9), torch.nan_to_num(codes, nan=1e9))
+
+
+def inputs(seed, tokens, heads, dim, dtype):
+    g = gen(seed)
+    x = torch.randn(tokens, heads, dim, generator=g) * torch.exp(2 * torch.randn(tokens, heads, 1, generator=g))
+    return x.to(dtype).cuda()
+
+
+@pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("heads, dim, bs, requests, longest", [
+    (8, 128, 16, 5, 1), (8, 128, 16, 7, 60), (2, 64, 32, 6, 100), (3, 256, 8, 5, 30), (1, 16, 64, 6, 150),
+    (5, 32, 128, 4, 300), (1, 128, 256, 3, 600), (16, 64, 1, 9, 4), (4, 256, 64, 40, 1), (2, 128, 2, 11, 9),
+    (1, 64, 16, 2, 1)])
+def test_append(cache, dtype, heads, dim, bs, requests, longest):
+    blocks = requests * (longest // bs + 2) + 2
+    runs = random_runs(heads * dim + bs, blocks, bs, requests, longest)
+    slots = runs_to_slots(runs, bs)
+    k, ks = filled_cache(1, blocks, bs, heads, dim, cache)
+    v, vs = filled_cache(2, blocks, bs, heads, dim, cache)
+    n = slots.numel()
+    check_append(inputs(3, n, heads, dim, dtype), inputs(4, n, heads, dim, dtype), k, v, ks, vs, slots)
+
+
+@pytest.mark.parametrize("cache", CACHES)
+def test_append_many_tokens(cache):
+    """Enough tokens that a CTA starts the runs of several tokens, with runs across the CTAs' ranges."""
+    blocks, bs, heads, dim = 700, 32, 8, 64
+    runs = random_runs(9, blocks, bs, 60, 700)
+    slots = runs_to_slots(runs, bs)
+    assert slots.numel() > 8000
+    k, ks = filled_cache(1, blocks, bs, heads, dim, cache)
+    v, vs = filled_cache(2, blocks, bs, heads, dim, cache)
+    n = slots.numel()
+    check_append(inputs(3, n, heads, dim, torch.bfloat16), inputs(4, n, heads, dim, torch.bfloat16), k, v, ks, vs, slots)
+
+
+@pytest.mark.parametrize("cache", CACHES)
+def test_append_one_token_at_a_time(cache):
+    """A page that fills token by token: its scale only grows, and every growth rounds the older tokens again."""
+    bs, heads, dim = 16, 2, 64
+    k, ks = filled_cache(1, 3, bs, heads, dim, cache)
+    v, vs = filled_cache(2, 3, bs, heads, dim, cache)
+    for i in range(2 * bs):
+        x = inputs(i, 1, heads, dim, torch.float16) * (1.3 ** (i % bs))
+        check_append(x, -x, k, v, ks, vs, torch.tensor([(1 + i // bs) * bs + i % bs], device="cuda"))
+        if i % bs:
+            assert (ks[1 + i // bs] >= grown).all()
+        grown = ks[1 + i // bs].clone()
+
+
+@pytest.mark.parametrize("cache", CACHES)
+def test_append_special_values(cache):
+    """Infinities, NaN, zeros, subnormals and the largest numbers; scales that the caller made are no powers of two."""
+    bs, heads, dim = 16, 2, 64
+    for dtype in (torch.float16, torch.bfloat16):
+        k, ks = filled_cache(1, 5, bs, heads, dim, cache)
+        v, vs = filled_cache(2, 5, bs, heads, dim, cache)
+        ks.mul_(1.37)
+        x = inputs(7, 4 * bs, heads, dim, dtype)
+        x[3, 0, 5], x[4, 1, 0], x[5, 1, 63] = float("inf"), float("-inf"), float("nan")
+        x[16:32] = 0
+        x[33:36] = torch.finfo(dtype).max
+        x[48:] = torch.finfo(dtype).smallest_normal / 8
+        slots = runs_to_slots([(0, 3, 13), (1, 0, 16), (2, 7, 9), (3, 0, 16)], bs)
+        check_append(x[:54], x[:54].flip(0).contiguous(), k, v, ks, vs, slots)
+
+
+def test_append_a_run_that_is_all_non_finite():
+    k, ks = filled_cache(1, 2, 16, 1, 64, E4M3)
+    v, vs = filled_cache(2, 2, 16, 1, 64, E4M3)
+    x = torch.full((3, 1, 64), float("inf"), dtype=torch.bfloat16, device="cuda")
+    x[1] = float("nan")
+    check_append(x, -x, k, v, ks, vs, torch.tensor([16, 17, 18], device="cuda"))
+    assert (ks[1] == 2.0 ** -126).all()
+
+
+@pytest.mark.parametrize("cache", CACHES)
+def test_append_strided(cache):
+    """Keys and values as slices of a fused projection; caches with padded rows, interleaved K and V and head-major pages."""
+    bs, heads, dim, blocks, n = 16, 4, 64, 6, 40
+    qkv = inputs(3, n, 3 * heads, dim, torch.float16)
+    odd = inputs(4, n, heads, dim + 1, torch.float16)[..., 1:]        # rows on odd addresses: copied
+    slots = torch.stack((runs_to_slots([(4, 5, 11), (None, 0, 1), (2, 0, 16), (0, 0, 12)], bs),) * 2, 1)[:, 0]
+    a, s = filled_cache(1, blocks, bs, heads, 2 * dim, cache)
+    scales = torch.stack((s, s * 2), 2)
+    check_append(qkv[:, heads:2 * heads], qkv[:, 2 * heads:], a[..., :dim], a[..., dim:], scales[..., 0], scales[..., 1],
+                 slots)
+    b, s = filled_cache(2, blocks, heads, bs, dim, cache)
+    b = b.transpose(1, 2)
+    c = filled_cache(3, 2 * blocks, bs, heads, dim, cache)[0]
+    check_append(odd, qkv[:, :heads], b, c[::2], scales[..., 1], torch.ones(heads, blocks, device="cuda").T, slots)
+
+
+def test_append_skips_slots_outside_and_leaves_other_pages():
+    bs, heads, dim, blocks = 16, 2, 64, 5
+    k, ks = filled_cache(1, blocks, bs, heads, dim, E4M3)
+    v, vs = filled_cache(2, blocks, bs, heads, dim, E4M3)
+    slots = torch.tensor([-1, 80, 2 ** 40, -2 ** 40, 33, 34, 79], dtype=torch.int64, device="cuda")
+    x = inputs(3, 7, heads, dim, torch.bfloat16)
+    check_append(x, x + 1, k, v, ks, vs, slots)
+    kept = [t.clone() for t in (k, v, ks, vs)]
+    fa_b200.paged_kv_append(x, x, k, v, ks, vs, torch.full((7,), -1, dtype=torch.int64, device="cuda"))
+    fa_b200.paged_kv_append(x[:0], x[:0], k, v, ks, vs, slots[:0])
+    for t, u in zip((k, v, ks, vs), kept):
+        assert bytes_equal(t, u)
+
+
+@pytest.mark.parametrize("slots", [[5, 5], [6, 5], [3, 7], list(range(8, 16)) + [15] * 40])
+def test_append_reports_slots_out_of_order(slots):
+    k, ks = filled_cache(1, 3, 16, 2, 64, E4M3)
+    v, vs = filled_cache(2, 3, 16, 2, 64, E4M3)
+    x = inputs(3, len(slots), 2, 64, torch.float16)
+    other = [t[1:].clone() for t in (k, v, ks, vs)]
+    fa_b200.paged_kv_append(x, x, k, v, ks, vs, torch.tensor(slots, device="cuda"))
+    with pytest.raises(RuntimeError, match="repeat or do not rise"):
+        fa_b200.check_status()
+    fa_b200.check_status()                      # reported once
+    for t, u in zip((k, v, ks, vs), other):
+        assert bytes_equal(t[1:].contiguous(), u)
+
+
+# ---------------------------------------------------------------------------------------------------
+# decode
+# ---------------------------------------------------------------------------------------------------
+def decode_case(seed, lens, heads_q, heads_kv, dim, bs, dtype, cache, spare=2):
+    g = gen(seed)
+    batch, width = len(lens), max(1, max(-(-n // bs) for n in lens))
+    blocks = sum(-(-n // bs) for n in lens) + spare
+    ids = torch.randperm(blocks, generator=g).tolist()
+    table = torch.full((batch, width), -1, dtype=torch.int32)
+    for b, n in enumerate(lens):
+        for j in range(-(-n // bs)):
+            table[b, j] = ids.pop()
+    k, ks = filled_cache(seed + 1, blocks, bs, heads_kv, dim, cache)
+    v, vs = filled_cache(seed + 2, blocks, bs, heads_kv, dim, cache)
+    ks.mul_(0.02)
+    q = torch.randn(batch, heads_q, dim, generator=g).to(dtype).cuda()
+    return [q, k, v, ks, vs, table.cuda(), ints(lens)]
+
+
+def check_decode(args, **kw):
+    got = fa_b200.flash_attention_decode_paged_8bit(*args, **kw)
+    want, bound = oracle.decode8_ref(*args, **kw)
+    assert got.dtype == args[0].dtype and got.shape == args[0].shape
+    half_step = torch.finfo(got.dtype).eps / 2
+    # the result's own rounding (below the normal range: half of the smallest step), on top of what the kernel may be off
+    allowed = bound * (1 + half_step) + want.abs() * half_step + torch.finfo(got.dtype).smallest_normal * half_step
+    excess = (got.double() - want).abs() - allowed
+    assert torch.isfinite(got).all()
+    assert (excess <= 0).all(), f"off by {(excess + allowed).max():.3e}, {(excess).max():.3e} more than allowed"
+    return got
+
+
+@pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lens, heads_q, heads_kv, dim, bs", [
+    ([1], 1, 1, 64, 16), ([256], 8, 8, 128, 16), ([1000, 3], 32, 8, 128, 16), ([77, 0, 300], 4, 2, 64, 8),
+    ([129, 128, 127], 16, 1, 128, 32), ([513], 10, 2, 256, 64), ([40, 900], 24, 8, 16, 16), ([65, 31], 15, 3, 32, 4),
+    ([700, 1, 64], 32, 2, 64, 1), ([333], 12, 12, 128, 128), ([50, 2000], 20, 4, 128, 256), ([257], 33, 1, 256, 16),
+    ([5, 6, 7, 8], 64, 4, 128, 2), ([1500], 40, 1, 128, 16), ([90, 91], 48, 16, 64, 16)])
+def test_decode(cache, dtype, lens, heads_q, heads_kv, dim, bs):
+    check_decode(decode_case(len(lens) * 7 + dim, lens, heads_q, heads_kv, dim, bs, dtype, cache))
+
+
+@pytest.mark.parametrize("lens", [[1], [16384], [20000, 17], [3218, 15003, 6237, 12772], list(range(0, 2400, 17)),
+                                  [31] * 300, [0] * 5, [4000] + [1] * 200])
+def test_decode_lengths(lens):
+    """Few long contexts, many short ones, and mixtures: every way in which the work is split and joined."""
+    check_decode(decode_case(3, lens, 16, 4, 64, 16, torch.float16, E4M3))
+    check_decode(decode_case(4, lens, 8, 1, 128, 16, torch.bfloat16, torch.int8))
+
+
+def test_decode_batch_of_thousands():
+    g = gen(1)
+    lens = torch.randint(0, 40, (1700,), generator=g).tolist()
+    check_decode(decode_case(5, lens, 4, 2, 64, 16, torch.float16, E4M3))
+
+
+@pytest.mark.parametrize("cache", CACHES)
+def test_decode_never_reads_behind_the_context_or_bad_pages(cache):
+    """NaN behind every context, in pages that no request holds and in their scales; ids out of range; lengths that
+    exceed the table or are negative."""
+    args = decode_case(6, [37, 160, 5, 48], 8, 2, 128, 16, torch.float16, cache)
+    q, k, v, ks, vs, table, lens = args
+    used = {int(p) for p in table.flatten().tolist() if p >= 0}
+    for t in (k, v):
+        raw = t.view(torch.uint8)
+        for p in range(t.shape[0]):
+            if p not in used:
+                raw[p] = 0x7f
+        for b, n in enumerate(lens.tolist()):
+            if n % 16:
+                raw[int(table[b, n // 16]), n % 16:] = 0x7f
+    for s in (ks, vs):
+        for p in range(k.shape[0]):
+            if p not in used:
+                s[p] = float("nan")
+    check_decode(args)
+    table[0, 1], table[1, 0], table[2, 0] = -1, k.shape[0], 10 ** 9
+    check_decode(args)
+    lens[1], lens[3] = 10 ** 9, -4
+    got = check_decode(args)
+    assert (got[2] == 0).all() and (got[3] == 0).all()
+
+
+def test_decode_scales_of_every_size():
+    """Value scales from 2^-126 to 2^100 between pages, zero scales, and scores that grow along the context."""
+    args = decode_case(7, [400, 250], 8, 2, 64, 16, torch.bfloat16, E4M3)
+    g = gen(2)
+    args[4].copy_(torch.exp2(torch.randint(-126, 101, args[4].shape, generator=g).float()))
+    check_decode(args)
+    args[4].zero_()
+    assert (fa_b200.flash_attention_decode_paged_8bit(*args) == 0).all()
+    args = decode_case(8, [600], 4, 1, 128, 16, torch.float16, torch.int8)
+    ramp = torch.linspace(0.1, 60, 38, device="cuda")
+    for j, p in enumerate(args[5][0].tolist()):
+        args[3][p] = ramp[j] * 0.01
+    check_decode(args)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.3, 1.0, 1e-6])
+def test_decode_softmax_scales(scale):
+    check_decode(decode_case(9, [200, 31], 8, 2, 128, 16, torch.bfloat16, E4M3), softmax_scale=scale)
+
+
+def test_decode_queries_of_every_size():
+    for factor in (1e-30, 1e-4, 1e20):
+        args = decode_case(10, [200, 31], 8, 2, 128, 16, torch.bfloat16, E4M3)
+        args[0] *= factor
+        args[3] /= factor
+        check_decode(args)
+
+
+def test_decode_nan_stays_in_its_row():
+    args = decode_case(11, [100, 100], 8, 2, 64, 16, torch.float16, E4M3)
+    clean = fa_b200.flash_attention_decode_paged_8bit(*args)
+    args[0][0, 3, 7] = float("nan")
+    got = fa_b200.flash_attention_decode_paged_8bit(*args)
+    assert torch.isnan(got[0, 3]).all()
+    rest = torch.ones(2, 8, dtype=torch.bool)
+    rest[0, 3] = False
+    assert torch.equal(got[rest], clean[rest])
+
+
+@pytest.mark.parametrize("cache", CACHES)
+def test_decode_strided(cache):
+    args = decode_case(12, [100, 333], 8, 4, 64, 16, torch.float16, cache)
+    q, k, v, ks, vs, table, lens = args
+    both = torch.cat((k.view(torch.uint8), v.view(torch.uint8)), -1).view(cache)          # K and V side by side
+    major = v.view(torch.uint8).transpose(1, 2).contiguous().transpose(1, 2).view(cache)   # head-major pages
+    qkv = torch.cat((q, q, q), 1)
+    want = fa_b200.flash_attention_decode_paged_8bit(*args)
+    scales = torch.stack((ks, vs), 2)
+    for kk, vv in ((both[..., :64], both[..., 64:]), (k, major), (both[..., :64], major)):
+        got = fa_b200.flash_attention_decode_paged_8bit(qkv[:, 8:16], kk, vv, scales[..., 0], scales[..., 1],
+                                                        table.T.contiguous().T, torch.stack((lens, lens), 1)[:, 1])
+        assert torch.equal(got, want)
+    odd = torch.zeros(2, 8, 65, dtype=q.dtype, device="cuda")[..., 1:]
+    odd.copy_(q)
+    assert torch.equal(fa_b200.flash_attention_decode_paged_8bit(odd, *args[1:]), want)
+
+
+def test_decode_one_page_for_many_requests():
+    """A prefix that requests share: the same page in several rows, and twice in one."""
+    args = decode_case(13, [64, 64, 64], 8, 2, 128, 16, torch.float16, E4M3)
+    args[5][1, :3] = args[5][0, :3]
+    args[5][2, 1] = args[5][2, 0]
+    check_decode(args)
+
+
+def test_decode_results_do_not_change_between_calls():
+    args = decode_case(14, [5000, 3, 700], 32, 8, 128, 16, torch.bfloat16, E4M3)
+    first = fa_b200.flash_attention_decode_paged_8bit(*args)
+    for _ in range(5):
+        assert torch.equal(fa_b200.flash_attention_decode_paged_8bit(*args), first)
+
+
+def test_decode_offsets_beyond_32_bits():
+    """A cache of more than 2^32 bytes, whose last pages hold the context."""
+    bs, heads, dim = 16, 8, 128
+    blocks = 2 ** 32 // (bs * heads * dim) + 40
+    small = decode_case(15, [300], 16, heads, dim, bs, torch.float16, torch.int8)
+    pages = small[1].shape[0]
+    k, v = (torch.zeros(blocks, bs, heads, dim, dtype=torch.int8, device="cuda") for _ in range(2))
+    ks, vs = (torch.ones(blocks, heads, device="cuda") for _ in range(2))
+    for big, little in zip((k, v, ks, vs), small[1:5]):
+        big[-pages:] = little
+    far = torch.where(small[5] >= 0, small[5] + (blocks - pages), small[5])
+    got = fa_b200.flash_attention_decode_paged_8bit(small[0], k, v, ks, vs, far, small[6])
+    assert torch.equal(got, fa_b200.flash_attention_decode_paged_8bit(*small))
+    x = inputs(1, 5, heads, dim, torch.float16)
+    slots = torch.arange((blocks - 1) * bs + 3, (blocks - 1) * bs + 8, device="cuda")
+    tail = [t[-1:].clone() for t in (k, v, ks, vs)]
+    fa_b200.paged_kv_append(x, -x, k, v, ks, vs, slots)
+    fa_b200.paged_kv_append(x, -x, *tail, slots - (blocks - 1) * bs)
+    for big, little in zip((k, v, ks, vs), tail):
+        assert bytes_equal(big[-1:].contiguous(), little)
+
+
+# ---------------------------------------------------------------------------------------------------
+# together
+# ---------------------------------------------------------------------------------------------------
+def packed(seed, new, pad, heads, dim, dtype):
+    return inputs(seed, sum(max(n, 0) for n in new) + pad, heads, dim, dtype)
+
+
+STEPS = [[40, 0, 7, 0], [1, 33, 1, 0], [1, 1, 1, 2], [-1, 1, 1, 1], [50, 1, -1, 1], [1, 1, 90, 1], [1, 1, 1, 1]]
+
+
+@pytest.mark.parametrize("cache", CACHES)
+def test_a_server_s_steps(cache):
+    """Prompts, steps, ends and new requests in the same rows, two layers: every step against the oracle's own state."""
+    heads, group, dim, bs, blocks = 2, 4, 64, 16, 24
+    c = fa_b200.PagedKVCache8(2, blocks, bs, heads, dim, 4, 8, dtype=cache)
+    for i, new in enumerate(STEPS):
+        pad = i % 3
+        state = oracle.plan_ref(c.context_lens.tolist(), new, c.block_table.cpu(), c.free_blocks.cpu(),
+                                int(c.free_count), sum(max(n, 0) for n in new) + pad, bs)
+        slots, cu = c.plan(ints(new), len(state[0]))
+        assert slots.tolist() == state[0] and cu.tolist() == state[1]
+        assert c.context_lens.tolist() == state[2] and int(c.free_count) == state[3]
+        for layer in range(2):
+            key, value = (packed(10 * i + j + 2 * layer, new, pad, heads, dim, torch.bfloat16) for j in range(2))
+            want = [oracle.append_ref(x, y[layer], s[layer], slots.tolist())
+                    for x, y, s in ((key, c.k_cache, c.k_scales), (value, c.v_cache, c.v_scales))]
+            c.append(layer, key, value, slots)
+            assert torch.equal(c.k_cache[layer].double(), want[0][0]) and torch.equal(c.v_scales[layer].double(), want[1][1])
+            q = inputs(100 + i, 4, heads * group, dim, torch.bfloat16)
+            got = c.decode(layer, q)
+            ref, bound = oracle.decode8_ref(q, c.k_cache[layer], c.v_cache[layer], c.k_scales[layer], c.v_scales[layer],
+                                            c.block_table, c.context_lens)
+            assert ((got.double() - ref).abs() <= bound * 1.004 + ref.abs() * 2.0 ** -8 + 1e-30).all()
+
+
+def test_the_8_bit_cache_stays_near_the_exact_one():
+    """What rounding costs: attention over the cache against attention over the 16-bit keys and values. An e4m3 code is
+    off by 2^-4 of its value at most, so values alone move a row by at most 2^-4 of sum p |v|, and a score by at most
+    2^-4 of sum |q k|; with q of size 0.05 that is under 0.3 here and the whole under 2^-4 + (e^0.6 - 1)."""
+    heads, dim, n = 2, 64, 500
+    c = fa_b200.PagedKVCache8(1, 40, 16, heads, dim, 1, 40)
+    slots, _ = c.plan(ints([n]), n)
+    key, value = inputs(1, n, heads, dim, torch.float16).clamp(-3, 3), inputs(2, n, heads, dim, torch.float16).clamp(-3, 3)
+    c.append(0, key, value, slots)
+    q = (torch.randn(1, 8, dim, generator=gen(3)) * 0.05).half().cuda()
+    got = c.decode(0, q, softmax_scale=1.0).double()
+    k, v = (x.double().repeat_interleave(4, 1) for x in (key, value))
+    sums = torch.einsum("hd,nhd->hn", q[0].double().abs(), k.abs()).max()
+    assert sums / 16 < 0.6
+    p = torch.softmax(torch.einsum("hd,nhd->hn", q[0].double(), k), -1)
+    want, weight = torch.einsum("hn,nhd->hd", p, v), torch.einsum("hn,nhd->hd", p, v.abs())
+    assert ((got[0] - want).abs() <= (2.0 ** -4 + 2 * (torch.exp(sums / 16) - 1)) * weight).all()
+
+
+def test_steps_captured_in_a_graph():
+    """A decode step as a CUDA graph: replays continue from the state that the step before left."""
+    heads, dim, bs = 2, 64, 16
+    live, ref = (fa_b200.PagedKVCache8(1, 30, bs, heads, dim, 3, 10) for _ in range(2))
+    start = ints([20, 3, 0])
+    x = inputs(1, 23, heads, dim, torch.float16)
+    for c in (live, ref):
+        slots, _ = c.plan(start, 23)
+        c.append(0, x, -x, slots)
+    new, key, q = ints([1, 1, 1]), inputs(2, 3, heads, dim, torch.float16), inputs(3, 3, 8, dim, torch.float16)
+
+    def step(c, key, q):
+        slots, _ = c.plan(new, 3)
+        c.append(0, key, key, slots)
+        return c.decode(0, q)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(fa_b200.PagedKVCache8(1, 30, bs, heads, dim, 3, 10), key, q)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(live, key, q)
+    for i in range(20):
+        key.copy_(inputs(50 + i, 3, heads, dim, torch.float16) * (1 + i))
+        graph.replay()
+        want = step(ref, key, q)
+        assert torch.equal(out, want), i
+    assert torch.equal(live.block_table, ref.block_table) and live.context_lens.tolist() == [40, 23, 20]
+    assert bytes_equal(live.k_cache, ref.k_cache) and torch.equal(live.k_scales, ref.k_scales)
+
+
+def test_two_streams_at_once():
+    a = decode_case(16, [9000, 50], 32, 8, 128, 16, torch.float16, E4M3)
+    b = decode_case(17, [400] * 40, 32, 8, 128, 16, torch.float16, E4M3)
+    want = [fa_b200.flash_attention_decode_paged_8bit(*x) for x in (a, b)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(fa_b200.flash_attention_decode_paged_8bit(*(a, b)[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(x, want[i]) for x in got[i])
+
+
+def test_ops_under_fake_tensors_and_opcheck():
+    d = decode_case(18, [40, 70], 8, 2, 64, 16, torch.float16, E4M3)
+    torch.library.opcheck(paged_cache._decode8_op, (*d, 0.125), test_utils="test_faketensor")
+    tests = ("test_schema", "test_faketensor")        # the schema check multiplies, which torch cannot do in e4m3
+    d = decode_case(18, [40, 70], 8, 2, 64, 16, torch.float16, torch.int8)
+    torch.library.opcheck(paged_cache._decode8_op, (*d, 0.125), test_utils=tests)
+    k, ks = filled_cache(1, 4, 16, 2, 64, torch.int8)
+    v, vs = filled_cache(2, 4, 16, 2, 64, torch.int8)
+    x = inputs(3, 4, 2, 64, torch.float16)
+    slots = torch.arange(4, device="cuda")
+    torch.library.opcheck(paged_cache._append_op, (x, x.clone(), k, v, ks, vs, slots), test_utils=tests)
+    torch.library.opcheck(paged_cache._plan_op, (*random_plan(1, 5, 16, 8, 20, 30), 16), test_utils=tests)
+
+
+def test_compiled_step_equals_the_eager_one():
+    d = decode_case(19, [40, 70], 8, 2, 64, 16, torch.float16, E4M3)
+    fn = torch.compile(lambda *t: fa_b200.flash_attention_decode_paged_8bit(*t) * 2, backend="aot_eager", fullgraph=True)
+    assert torch.equal(fn(*d), fa_b200.flash_attention_decode_paged_8bit(*d) * 2)
+
+
+def test_inference_only():
+    d = decode_case(20, [40], 8, 2, 64, 16, torch.float16, E4M3)
+    d[0].requires_grad_(True)
+    with pytest.raises(RuntimeError, match="inference-only"):
+        fa_b200.flash_attention_decode_paged_8bit(*d)
+    with torch.no_grad():
+        fa_b200.flash_attention_decode_paged_8bit(*d)
