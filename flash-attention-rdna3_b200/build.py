@@ -3,7 +3,8 @@
 Usage: python flash-attention-rdna3_b200/build.py [--force] [--verbose] [--prof] [--debug-bounds]
 
 Each .cu file is compiled to an object only when it or a header is newer than the object, then all
-objects are linked into fa_b200/libfa_b200.so next to the Python package that loads it.
+objects are linked into fa_b200/libfa_b200.so next to the Python package that loads it. g++ then builds
+fa_b200/_paged_native.so, the Python binding of the paged-cache calls.
 
 --prof builds a second library, fa_b200/libfa_b200_prof.so, with -DFA_PROF: the tensor-core forward, backward and decode
 kernels then count, per CTA and role, the cycles spent in each phase of their loops (csrc/fa_prof.cuh) and the library
@@ -25,6 +26,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "build")
 OUT = os.path.join(HERE, "fa_b200", "libfa_b200.so")
+BINDING = os.path.join(HERE, "fa_b200", "_paged_native.so")
 SOURCES = ["fa_api.cu", "fa_simt.cu", "fa_tiled_fwd.cu", "fa_tiled_dq.cu", "fa_tiled_dkdv.cu", "fa_decode.cu", "fa_tiny.cu", "fa_fwd_sm100.cu", "fa_bwd_sm100.cu", "fa_wide_sm100.cu", "fa_decode_sm100.cu", "fa_paged8_cache.cu", "fa_paged8_decode.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-std=c++17", "-lineinfo",
@@ -82,7 +84,32 @@ def build(force=False, verbose=False, prof=False, debug_bounds=False):
         if r.returncode != 0:
             sys.stderr.write(r.stdout + r.stderr)
             raise RuntimeError("link failed")
+    if not prof and not debug_bounds:
+        _build_binding(force, verbose, header_time)
     return OUT
+
+
+def _build_binding(force, verbose, header_time):
+    """The Python binding of the paged-cache calls (csrc/fa_paged8_bind.cpp), a module against torch's C++ headers."""
+    src = os.path.join(CSRC, "fa_paged8_bind.cpp")
+    if not force and os.path.exists(BINDING) and os.path.getmtime(BINDING) >= max(os.path.getmtime(src), header_time):
+        return
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++20", "-shared", "-fPIC", "-fvisibility=hidden", src, "-o", BINDING,
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f"-I{sysconfig.get_paths()['include']}",
+           *(f"-isystem{d}" for d in cpp_extension.include_paths("cuda")), f"-L{lib}",
+           "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-Wl,--as-needed"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if verbose or r.returncode != 0:
+        sys.stderr.write(f"--- fa_paged8_bind.cpp\n{r.stdout}{r.stderr}\n")
+    if r.returncode != 0:
+        raise RuntimeError("compiling fa_paged8_bind.cpp failed")
 
 
 if __name__ == "__main__":

@@ -5,36 +5,42 @@
 // with ks_t, vs_t the scales of the page that holds token t. One pass over the cache with running m and sums; every byte
 // is read once for all query heads of its kv head, so the bound is HBM: 2 * head_dim bytes a token and kv head.
 //
-// A warp owns one kv head and streams tiles of 8 KB (64, 32 or 16 tokens of K and V at head dims 64, 128, 256) through a
-// ring of its own in shared memory, filled with cp.async; no warp waits for another inside the loop. Both products run on
+// One CTA an SM: a producer warp brings tiles of 64 KB (64, 32 or 16 tokens of 8 heads at head dims 64, 128, 256; of fewer
+// heads, accordingly more tokens) into a ring of three stages, one TMA box of up to 16 tokens x heads for each page and
+// operand; eight compute warps own one kv head each (with fewer heads, a share of its tokens). Both products run on
 // m16n8k16 fp16 MMAs with tokens (then dimensions) as the 16 rows and up to 8 query heads as the 8 columns: a tensor
 // tile of 128 rows would be 15/16 empty at these group sizes. The codes are widened to fp16 in registers, exactly.
 //
-// The work of the whole batch is one line of units (a tile for every warp of the CTA), cut into equal stretches, one for
-// each SM, wherever the sequences begin and end: ragged batches keep all SMs busy with no knowledge of the lengths on the
-// host. A stretch that covers a whole item (request, heads of a CTA) writes the output; one that covers part of it writes
-// its sums to the workspace, and paged8_merge_kernel joins the parts in the order of the stretches.
+// The work of the whole batch is one line of units (tiles), cut into equal stretches, one for each SM, wherever the
+// sequences begin and end: ragged batches keep all SMs busy with no knowledge of the lengths on the host. A stretch that
+// covers a whole item (request, heads of a CTA) writes the output; one that covers part of it writes its sums to the
+// workspace, and paged8_merge_kernel joins the parts in the order of the stretches.
+#include <cuda.h>
+
 #include "fa_paged8.cuh"
+#include "fa_sm100.cuh"
+#include "fa_tma_host.h"
 
 namespace fa {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
-constexpr int kTileBytes = 8192;  // K and V of one warp's tile
+constexpr int kWarps = 8;                       // compute warps; one more loads
+constexpr int kThreads = kWarps * 32 + 32;
+constexpr int kStageBytes = 65536;              // K, then V
 constexpr int kStages = 3;
 constexpr int kMaxCtas = 256;
+constexpr int kMergeThreads = 256;
+constexpr float kSlack = 10.f;                  // log2 of what a score may pass the softmax reference by
+constexpr uint32_t kNoPage = 0x7fffbad0u;       // K scale (a NaN of its own) of tokens whose page id is out of range
 
 struct Args {
-  int dtype, batch, heads_q, heads_kv, head_dim, group;
+  int dtype, batch, heads_q, head_dim, group;
   int num_blocks, max_blocks, shift;
-  int head_ctas, row_chunks, warps_per_head;  // items of a request = heads_kv / heads a CTA * chunks of query heads
+  int head_ctas, row_chunks;         // items of a request = groups of heads * chunks of query heads
+  int head_shift;                    // log2 of the kv heads of a CTA
+  int box_shift, scale_shift;        // log2 of the tokens of a TMA box (at most 16), of a scale entry (at most 8)
   const void* q;
   int64_t q_sb, q_sh;
-  const uint8_t* k;
-  const uint8_t* v;
-  uint32_t k_sb, k_st, v_sb, v_st;  // bytes
-  int64_t k_sh, v_sh;
   const float* ks;
   const float* vs;
   int64_t ks_sb, ks_sh, vs_sb, vs_sh;
@@ -45,7 +51,8 @@ struct Args {
   void* out;
   int64_t o_sb, o_sh;
   float scale_log2;
-  int64_t* prefix;   // batch + 1: first unit of every request
+  int32_t* status;
+  int4* cuts;        // for every CTA: request, item, first CTA and number of CTAs of the item that its stretch begins inside
   float* part_stat;  // (2 * CTAs, rows of a CTA, 2): m, l
   float* part_o;     // (2 * CTAs, rows of a CTA, D)
 };
@@ -54,19 +61,18 @@ struct Args {
 __host__ __device__ constexpr int item_rows(int heads_per_cta, int nt) { return heads_per_cta * nt * 8; }
 
 template <int D> struct Tile {
-  static constexpr int kTokens = kTileBytes / (2 * D);
+  static constexpr int kTokens = 4096 / D;            // tokens of a compute warp in a stage
   static constexpr int kMt = kTokens / 16;            // 16-token tiles
-  static constexpr int kPages = kTokens > 32 ? 2 : 1; // page ids that a lane holds
-  static constexpr int kLanes = D / 16;               // lanes a row in a 16-byte copy
+  static constexpr int kRow = D < 128 ? D : 128;      // bytes of a row in shared memory (256 dimensions: two half tiles)
+  static constexpr int kHalves = D / kRow;
 };
 
-// Byte offset of a 16-byte chunk of a row. The XOR spreads both access patterns over the banks: K reads four neighbouring
-// chunks of the rows r and r ^ 5, V two neighbouring chunks of four even (or four odd) rows.
+// Rows of 128 (64) bytes lie in the 128-byte (64-byte) TMA swizzle: 16-byte chunk c of the row at offset x is chunk
+// c ^ (bits 7 .. 9 (7 .. 8) of x).
 template <int D>
-__device__ __forceinline__ int chunk_at(int row, int chunk) {
-  return row * D + ((D == 64 ? chunk ^ ((row >> 1) & 3) : chunk ^ (row & 7)) << 4);
-}
-// token of an MMA row: a permutation that makes the reads above free of bank conflicts (tokens are summed over)
+__device__ __forceinline__ uint32_t swizzle_of(uint32_t x) { return ((x >> 7) & (D == 64 ? 3u : 7u)) << 4; }
+// token of an MMA row: a permutation (tokens are summed over) with which the K reads (four neighbouring chunks of the rows
+// r, r ^ 5) and the V reads (two chunks of four even or four odd rows) of a quarter warp touch every bank once
 __device__ __forceinline__ int token_of(int m) { return m ^ ((m & 1) << 2); }
 
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -80,7 +86,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ uint4 lds128(uint32_t a) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
@@ -91,13 +96,13 @@ __device__ __forceinline__ uint2 lds64(uint32_t a) {
   asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
   return v;
 }
-// copies of `bytes` (0 or all) with the rest zero: rows that are not there become zeros, NaN patterns behind a context
-// never reach the products
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ void copy4(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+__device__ __forceinline__ float lds_f32(uint32_t a) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a));
+  return v;
 }
 __device__ __forceinline__ void head_barrier(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
@@ -130,33 +135,62 @@ struct Cursor {
   }
 };
 
-template <int D, int NT> struct Smem {
-  static constexpr int kRing = kWarps * kStages * kTileBytes;
-  static constexpr int kScaleStage = Tile<D>::kTokens * 8 + 8;  // K scales, V scales, two mask words
-  static constexpr int kScales = kWarps * kStages * kScaleStage;
-  static constexpr int kMerge = kWarps * 2048;
-  static constexpr int kStats = kWarps * NT * 8 * 16;
-  static constexpr int kBytes = kRing + kScales + kMerge + kStats;
+// Stretches: the first `more` CTAs take base + 1 units, the others base.
+struct Stretches {
+  int64_t base, more;
+  __device__ __forceinline__ int64_t begin(int64_t i) const { return i * base + min(i, more); }
+  __device__ __forceinline__ int cta_of(int64_t unit) const {
+    const int64_t long_part = more * (base + 1);
+    return (int)(unit < long_part ? unit / (base + 1) : more + (unit - long_part) / base);
+  }
 };
 
+template <int D, int NT> struct Smem {
+  static constexpr int kRing = kStages * kStageBytes;
+  static constexpr int kScaleStage = Tile<D>::kTokens * kWarps * 8;  // K and V scales of a stage, at one token an entry
+  static constexpr int kScales = kStages * kScaleStage;
+  static constexpr int kMerge = kWarps * 2048;
+  static constexpr int kStats = kWarps * NT * 8 * 8;
+  static constexpr int kBytes = kRing + kScales + kMerge + kStats + 1024;  // the ring is moved to a 1024-byte boundary
+};
+
+// Waits for a phase; a wait that runs out is recorded, and later ones are not begun.
+__device__ __forceinline__ void wait_for(uint64_t* bar, uint32_t parity, bool& lost, int32_t* status) {
+  if (lost || mbar_wait(bar, parity)) return;
+  lost = true;
+  if (status != nullptr) *status = 1;
+}
+
 template <typename C8, int D, int NT>
-__global__ void __launch_bounds__(kThreads, 1) paged8_kernel(const Args a) {
+__global__ void __launch_bounds__(kThreads, 1)
+    paged8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const Args a) {
   using T = Tile<D>;
-  constexpr int kTokens = T::kTokens, kMt = T::kMt, kJ = D / 64, kNm = D / 16, kRows = NT * 8;
+  constexpr int kTokens = T::kTokens, kMt = T::kMt, kJ = D / 64, kNm = D / 16, kRows = NT * 8, kRow = T::kRow;
   constexpr int kRoundTiles = NT == 1 ? 4 : 2, kCols = kRoundTiles * 16;  // columns of a merge round
-  extern __shared__ __align__(128) uint8_t smem[];
+  constexpr int kHalfBytes = kStageBytes / 2 / T::kHalves;
+  extern __shared__ uint8_t smem_raw[];
   __shared__ int64_t scan_s[kWarps + 1];
   __shared__ int64_t start_s[2];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
-  const int heads_cta = kWarps / a.warps_per_head, wh = warp / a.warps_per_head, wt = warp % a.warps_per_head;
-  const int span = kTokens * a.warps_per_head, items = a.head_ctas * a.row_chunks;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  __shared__ __align__(8) uint64_t full_s[kStages], empty_s[kStages];
+  __shared__ int plain_s[kStages];  // whether every token of the stage is there
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int heads_cta = 1 << a.head_shift, warps_head = kWarps >> a.head_shift;
+  const int span = kTokens * warps_head, items = a.head_ctas * a.row_chunks;
+  uint8_t* smem = smem_raw + ((1024u - smem_u32(smem_raw)) & 1023u);
+  grid_launch_dependents();
+  if (tid == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&full_s[i], 33);  // the producer's lanes (scales) and its word that everything is on the way
+      mbar_init(&empty_s[i], kWarps);
+    }
+    mbar_fence_init();
+  }
 
   // ---- this CTA's stretch of units
   int64_t total, u_begin, u_end;
-  int ctas;
+  Stretches cut_line;
   {
-    const int per = (a.batch + kThreads - 1) / kThreads, b0 = min(tid * per, a.batch), b1 = min(b0 + per, a.batch);
+    const int per = (a.batch + kWarps * 32 - 1) / (kWarps * 32), b0 = min(tid * per, a.batch), b1 = min(b0 + per, a.batch);
     int64_t mine = 0;
     for (int b = b0; b < b1; ++b) mine += (int64_t)((clamped_len(a, b) + span - 1) / span) * items;
     int64_t sum = mine;
@@ -168,135 +202,186 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_kernel(const Args a) {
     if (lane == 31) scan_s[warp] = sum;
     __syncthreads();
     total = 0;
-    for (int w = 0; w < kWarps; ++w) {
+#pragma unroll
+    for (int w = 0; w <= kWarps; ++w) {
       if (w < warp) sum += scan_s[w];
       total += scan_s[w];
     }
-    ctas = (int)min((int64_t)gridDim.x, total);
+    const int ctas = (int)min((int64_t)gridDim.x, total);
     u_begin = u_end = 0;
     if ((int)blockIdx.x < ctas) {
-      u_begin = blockIdx.x * total / ctas;
-      u_end = (blockIdx.x + 1) * total / ctas;
+      if (total <= UINT32_MAX) {
+        cut_line.base = (uint32_t)total / (uint32_t)ctas;
+      } else {
+        cut_line.base = total / ctas;
+      }
+      cut_line.more = total - cut_line.base * ctas;
+      u_begin = cut_line.begin(blockIdx.x);
+      u_end = cut_line.begin(blockIdx.x + 1);
     }
     int64_t at = sum - mine;
-    const bool here = mine > 0 && at <= u_begin && u_begin < sum;
-    if (here || blockIdx.x == 0) {
+    if (u_begin < u_end && at <= u_begin && u_begin < sum) {
       for (int b = b0; b < b1; ++b) {
         const int64_t n = (int64_t)((clamped_len(a, b) + span - 1) / span) * items;
-        if (blockIdx.x == 0) a.prefix[b] = at;
-        if (here && at <= u_begin && u_begin < at + n) {
+        if (at <= u_begin && u_begin < at + n) {
           start_s[0] = b;
           start_s[1] = at;
         }
         at += n;
       }
     }
-    if (blockIdx.x == 0 && tid == 0) a.prefix[a.batch] = total;
     __syncthreads();
   }
+  const int units = (int)(u_end - u_begin);
+  Cursor at;
+  if (units > 0) {
+    at.b = (int)start_s[0];
+    at.enter(a, span);
+    const int64_t rest = u_begin - start_s[1];
+    if (rest < INT32_MAX) {
+      at.item = (int)rest / at.steps;
+      at.step = (int)rest % at.steps;
+    } else {
+      at.item = (int)(rest / at.steps);
+      at.step = (int)(rest % at.steps);
+    }
+  }
+  bool lost = false;
+
+  if (warp == kWarps) {
+    // =============================== producer warp ===============================
+    const int box = 1 << a.box_shift, boxes = span >> a.box_shift, in_page = (1 << a.shift) - 1;
+    const int entries = (span >> a.scale_shift) << a.head_shift;
+    const uint32_t box_bytes = (uint32_t)(box << a.head_shift) * kRow;
+    auto page_at = [&](int pos) -> int {
+      if (pos >= at.len) return -1;
+      const int id = a.table[at.b * a.bt_sb + (pos >> a.shift) * a.bt_sk];
+      return id >= 0 && id < a.num_blocks ? id : -1;
+    };
+    auto fetch = [&]() -> int { return lane < boxes ? page_at(at.step * span + lane * box) : -1; };
+    int page = -1;
+    if (units > 0) {
+      page = fetch();
+      if (lane == 0) {
+        tma_prefetch_desc(&k_map);
+        tma_prefetch_desc(&v_map);
+      }
+    }
+    int stage = 0, issued = 0;
+    uint32_t parity = 1;
+    for (; issued < units; ++issued) {
+      if (issued >= kStages) wait_for(&empty_s[stage], parity, lost, a.status);
+      lost = __any_sync(0xffffffffu, lost);
+      if (lost) break;
+      const int head0 = (at.item / a.row_chunks) << a.head_shift, pos0 = at.step * span;
+      uint8_t* kt = smem + stage * kStageBytes;
+      const uint32_t st = smem_u32(smem) + Smem<D, NT>::kRing + stage * Smem<D, NT>::kScaleStage;
+      if (lane == 0)
+        asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(&full_s[stage])), "n"(kStageBytes) : "memory");
+      __syncwarp();
+      bool plain = true;
+      for (int i = lane; i < boxes; i += 32) {
+        const int pos = pos0 + i * box, id = i < 32 ? page : page_at(pos);
+        plain = plain && id >= 0 && pos + box <= at.len;
+        // tokens behind the context and pages out of range: a page behind the last one, which reads as zeros
+        const int c3 = id >= 0 ? id : a.num_blocks;
+#pragma unroll
+        for (int h = 0; h < T::kHalves; ++h) {
+          tma_load_4d(kt + h * kHalfBytes + i * box_bytes, &k_map, &full_s[stage], h * 128, pos & in_page, head0, c3);
+          tma_load_4d(kt + kStageBytes / 2 + h * kHalfBytes + i * box_bytes, &v_map, &full_s[stage], h * 128, pos & in_page, head0, c3);
+        }
+      }
+      plain = __all_sync(0xffffffffu, plain);
+      for (int e0 = 0; e0 < entries; e0 += 32) {
+        const int e = e0 + lane, pos = pos0 + ((e >> a.head_shift) << a.scale_shift);
+        int id = __shfl_sync(0xffffffffu, page, ((pos - pos0) >> a.box_shift) & 31);
+        if (boxes > 32) id = page_at(pos);
+        if (e >= entries) continue;
+        const uint32_t k_to = st + e * 4, v_to = k_to + entries * 4;
+        const int head = head0 + (e & (heads_cta - 1));
+        if (id >= 0) {
+          copy4(k_to, a.ks + id * a.ks_sb + head * a.ks_sh);
+          copy4(v_to, a.vs + id * a.vs_sb + head * a.vs_sh);
+        } else {
+          asm volatile("st.shared.u32 [%0], %1;" ::"r"(k_to), "r"(kNoPage) : "memory");
+          asm volatile("st.shared.u32 [%0], %1;" ::"r"(v_to), "r"(0) : "memory");
+        }
+      }
+      if (lane == 0) plain_s[stage] = plain;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&full_s[stage]);
+      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&full_s[stage])) : "memory");
+      if (issued + 1 < units) {
+        at.advance(a, span, items);
+        page = fetch();
+      }
+      if (++stage == kStages) {
+        stage = 0;
+        parity ^= 1;
+      }
+    }
+    if (lost) {  // copies on the way land before the CTA leaves
+      bool ignored = false;
+      for (int i = max(0, issued - kStages); i < issued; ++i) wait_for(&full_s[i % kStages], (i / kStages) & 1, ignored, a.status);
+    }
+    return;
+  }
+
   // empty contexts have no unit: their rows are zeros
   for (int b = blockIdx.x; b < a.batch; b += gridDim.x)
     if (clamped_len(a, b) == 0)
-      for (int i = tid; i < a.heads_q * (a.head_dim / 2); i += kThreads)
+      for (int i = tid; i < a.heads_q * (a.head_dim / 2); i += kWarps * 32)
         reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + b * a.o_sb + (i / (a.head_dim / 2)) * a.o_sh)[i % (a.head_dim / 2)] = 0u;
-  if (u_begin == u_end) return;
-
-  const uint32_t ring = smem_u32(smem) + warp * kStages * kTileBytes;
-  const uint32_t scales = smem_u32(smem) + Smem<D, NT>::kRing + warp * kStages * Smem<D, NT>::kScaleStage;
-  float* merge = reinterpret_cast<float*>(smem + Smem<D, NT>::kRing + Smem<D, NT>::kScales);
-  float4* stats = reinterpret_cast<float4*>(smem + Smem<D, NT>::kRing + Smem<D, NT>::kScales + Smem<D, NT>::kMerge);
-
-  Cursor put;
-  put.b = (int)start_s[0];
-  put.enter(a, span);
-  {
-    const int64_t rest = u_begin - start_s[1];
-    put.item = (int)(rest / put.steps);
-    put.step = (int)(rest % put.steps);
+  if (tid == 0) {
+    int4 cut = make_int4(0, 0, 0, 0);
+    if (units > 0 && at.step > 0) {
+      const int64_t begin = u_begin - at.step;
+      const int c0 = cut_line.cta_of(begin), c1 = cut_line.cta_of(begin + at.steps - 1);
+      cut = make_int4(at.b, at.item, c0, c1 - c0 + 1);
+    }
+    a.cuts[blockIdx.x] = cut;
   }
-  Cursor get = put;
-  const int units = (int)(u_end - u_begin);
 
-  // ---- producer side: page ids of the next tile are fetched one tile ahead of its copies
-  int page[T::kPages];
-  auto fetch_pages = [&]() {
-#pragma unroll
-    for (int i = 0; i < T::kPages; ++i) {
-      const int pos = put.step * span + wt * kTokens + lane + 32 * i;
-      page[i] = -1;
-      if (pos < put.len && lane + 32 * i < kTokens) {
-        const int id = a.table[put.b * a.bt_sb + (pos >> a.shift) * a.bt_sk];
-        if (id >= 0 && id < a.num_blocks) page[i] = id;
-      }
-    }
+  // =============================== compute warps ===============================
+  const int g = lane >> 2, t4 = lane & 3;
+  const int wh = warp >> (3 - a.head_shift), wt = warp & (warps_head - 1);
+  float* merge = reinterpret_cast<float*>(smem + Smem<D, NT>::kRing + Smem<D, NT>::kScales);
+  float2* stats = reinterpret_cast<float2*>(smem + Smem<D, NT>::kRing + Smem<D, NT>::kScales + Smem<D, NT>::kMerge);
+  // A box holds its tokens head by head, so token t (of the stage) of head h lies at row
+  // (t / box) * box * heads + h * box + t % box: 16 tokens further is 16 * heads rows, 8 tokens is 8 rows inside a box of
+  // 16 and 8 * heads rows otherwise, and the 8 tokens of a group differ by lane constants.
+  const int box = 1 << a.box_shift;
+  const uint32_t step16 = (uint32_t)(16 << a.head_shift) * kRow;
+  const uint32_t step8 = box == 16 ? 8u * kRow : (uint32_t)(8 << a.head_shift) * kRow;
+  auto lane_row = [&](int t) -> uint32_t {  // byte offset of token t < 8 of a group
+    return (uint32_t)(((t >> a.box_shift << a.box_shift) << a.head_shift) + wh * box + (t & (box - 1))) * kRow;
   };
-  auto issue = [&](int stage) {
-    const int head = (put.item / a.row_chunks) * heads_cta + wh;
-    const uint32_t kt = ring + stage * kTileBytes, vt = kt + kTileBytes / 2;
-    const uint32_t st = scales + stage * Smem<D, NT>::kScaleStage;
-    uint32_t mask[T::kPages];
-#pragma unroll
-    for (int i = 0; i < T::kPages; ++i) {
-      mask[i] = __ballot_sync(0xffffffffu, page[i] >= 0);
-      const int64_t id = max(page[i], 0);
-      const int bytes = page[i] >= 0 ? 4 : 0;
-      if (lane + 32 * i < kTokens) {
-        copy4(st + (lane + 32 * i) * 4, a.ks + id * a.ks_sb + head * a.ks_sh, bytes);
-        copy4(st + (kTokens + lane + 32 * i) * 4, a.vs + id * a.vs_sb + head * a.vs_sh, bytes);
-      }
-      if (lane == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(st + kTokens * 8 + i * 4), "r"(mask[i]) : "memory");
-    }
-    const int row0 = lane / T::kLanes, chunk = lane % T::kLanes;
-    const uint8_t* kh = a.k + head * a.k_sh + chunk * 16;
-    const uint8_t* vh = a.v + head * a.v_sh + chunk * 16;
-    const uint32_t within = (1u << a.shift) - 1;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int tok = j * (32 / T::kLanes) + row0;
-      const int i = j * (32 / T::kLanes) / 32;
-      const uint32_t id = max(__shfl_sync(0xffffffffu, page[i], tok & 31), 0);
-      const uint32_t in_page = (put.step * span + wt * kTokens + tok) & within;
-      const int bytes = ((mask[i] >> (tok & 31)) & 1) && chunk * 16 < a.head_dim ? 16 : 0;
-      const int at = chunk_at<D>(tok, chunk);
-      copy16(kt + at, kh + (uint64_t)id * a.k_sb + (uint64_t)in_page * a.k_st, bytes);
-      copy16(vt + at, vh + (uint64_t)id * a.v_sb + (uint64_t)in_page * a.v_st, bytes);
-    }
-  };
-  int put_left = units;
-  auto produce = [&](int stage) {
-    if (put_left > 0) {
-      issue(stage);
-      if (--put_left > 0) {
-        put.advance(a, span, items);
-        fetch_pages();
-      }
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
-  fetch_pages();
-#pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) produce(s);
+  const uint32_t warp_base = smem_u32(smem) + wt * kMt * step16;
+  const uint32_t k_row = lane_row(token_of(g)), va_row = lane_row(token_of(2 * t4)), vb_row = lane_row(token_of(2 * t4 + 1));
+  const uint32_t k_swz = swizzle_of<D>(k_row), va_swz = swizzle_of<D>(va_row), vb_swz = swizzle_of<D>(vb_row);
+  const uint32_t scale8 = (uint32_t)((8 >> a.scale_shift) << a.head_shift) * 4;
+  const uint32_t scale_base = smem_u32(smem) + Smem<D, NT>::kRing + wt * kMt * 2 * scale8 +
+                              (((token_of(g) >> a.scale_shift) << a.head_shift) + wh) * 4;
+  const uint32_t v_scales = (uint32_t)((span >> a.scale_shift) << a.head_shift) * 4;
 
-  // ---- consumer side
   uint32_t qf[NT][kJ * 4][2];
   float row_scale[NT][2];       // of rows 2 t4, 2 t4 + 1: softmax scale * log2(e) * the query row's own scale
   float o[NT][kNm][4], m[NT][2], l[NT][2];
   float vref = 0.f;             // power of two that the products with V are relative to
-  int begin_step = 0;
-
-  int stage = 0, fill = kStages - 1;
+  int begin_step = 0, stage = 0;
+  uint32_t parity = 0;
   for (int u = 0; u < units; ++u) {
-    const int head = (get.item / a.row_chunks) * heads_cta + wh, chunk0 = (get.item % a.row_chunks) * kRows;
-    if (u == 0 || get.step == 0) {
+    const int head = ((at.item / a.row_chunks) << a.head_shift) + wh, chunk0 = (at.item % a.row_chunks) * kRows;
+    if (u == 0 || at.step == 0) {
       // A new item: query rows as fp16 operands. fp16 rows go as they are; a bf16 row is first scaled by the power of
       // two that puts its largest value into [2^14, 2^15), which keeps every bit down to 2^-28 of that value.
-      begin_step = get.step;
+      begin_step = at.step;
       vref = __uint_as_float(1u << 23);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const int r = chunk0 + nt * 8 + g;
         const bool in = r < a.group;
-        const int64_t base = get.b * a.q_sb + (int64_t)(head * a.group + (in ? r : 0)) * a.q_sh;
+        const int64_t base = at.b * a.q_sb + (int64_t)(head * a.group + (in ? r : 0)) * a.q_sh;
         uint4 raw[kJ][2];
         float amax = 0.f;
 #pragma unroll
@@ -362,13 +447,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_kernel(const Args a) {
       }
     }
 
-    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
-    __syncwarp();
-    produce(fill);
-    fill = fill + 1 == kStages ? 0 : fill + 1;
-
-    const uint32_t kt = ring + stage * kTileBytes, vt = kt + kTileBytes / 2;
-    const uint32_t st = scales + stage * Smem<D, NT>::kScaleStage;
+    wait_for(&full_s[stage], parity, lost, a.status);
+    const bool plain = plain_s[stage] != 0;
+    const uint32_t kt = warp_base + stage * kStageBytes, vt = kt + kStageBytes / 2;
+    const uint32_t st = scale_base + stage * Smem<D, NT>::kScaleStage;
+    const int left = at.len - (at.step * span + wt * kTokens);  // tokens of the context from this tile's first on
     // ---- scores: rows are tokens, columns query heads
     float s[kMt][NT][4];
 #pragma unroll
@@ -377,10 +460,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_kernel(const Args a) {
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int c = 0; c < 4; ++c) s[mt][nt][c] = 0.f;
-      const int r = mt * 16 + token_of(g);
+      const uint32_t row = kt + mt * step16 + k_row;
 #pragma unroll
       for (int j = 0; j < kJ; ++j) {
-        const uint4 ka = lds128(kt + chunk_at<D>(r, t4 + 4 * j)), kb = lds128(kt + chunk_at<D>(r + 8, t4 + 4 * j));
+        const uint32_t chunk = ((uint32_t)((t4 + 4 * (j & 1)) << 4) ^ k_swz) + (j >> 1) * kHalfBytes;
+        const uint4 ka = lds128(row + chunk), kb = lds128(row + step8 + chunk);
         const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -390,73 +474,84 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_kernel(const Args a) {
         }
       }
     }
-    // ---- scales, mask, running maximum
-    float m_new[NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) m_new[nt][0] = m[nt][0], m_new[nt][1] = m[nt][1];
+    // ---- Scales and mask. m is a reference, not the maximum: it moves (with everything summed so far) only when a score
+    // passes it by more than 2^kSlack, so most tiles need no reduction over the warp. The products with V take p * vs
+    // relative to a power of two vref, which follows the page scales in the same way. What enters them is below
+    // 2^(kSlack + 2) and relative to the largest score and scale no less exact than with the maximum itself.
     float v_scale[kMt][2];
-    uint32_t v_top = 0u;
+    float excess = -1.f;
+    const uint32_t v_limit = __float_as_uint(vref) + (2u << 23);
+    bool v_moves = false;
 #pragma unroll
     for (int mt = 0; mt < kMt; ++mt) {
-      const int r = mt * 16 + token_of(g);
-      float k0, k1;
-      uint32_t mask;
-      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(k0) : "r"(st + r * 4));
-      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(k1) : "r"(st + (r + 8) * 4));
-      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v_scale[mt][0]) : "r"(st + (kTokens + r) * 4));
-      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v_scale[mt][1]) : "r"(st + (kTokens + r + 8) * 4));
-      asm volatile("ld.shared.u32 %0, [%1];" : "=r"(mask) : "r"(st + kTokens * 8 + (mt / 2) * 4));
-      const bool in0 = (mask >> (r & 31)) & 1, in1 = (mask >> ((r + 8) & 31)) & 1;
-      v_top = max(v_top, max(__float_as_uint(v_scale[mt][0]) & 0x7fffffffu, __float_as_uint(v_scale[mt][1]) & 0x7fffffffu));
+      const uint32_t at0 = st + mt * 2 * scale8, at1 = at0 + scale8;
+      const float k0 = lds_f32(at0), k1 = lds_f32(at1);
+      v_scale[mt][0] = lds_f32(at0 + v_scales);
+      v_scale[mt][1] = lds_f32(at1 + v_scales);
+      v_moves = v_moves || (__float_as_uint(v_scale[mt][0]) & 0x7fffffffu) >= v_limit ||
+                (__float_as_uint(v_scale[mt][1]) & 0x7fffffffu) >= v_limit;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float& x = s[mt][nt][e];
-          float& y = s[mt][nt][2 + e];
-          x = in0 ? x * (k0 * row_scale[nt][e]) : kNegInf;
-          y = in1 ? y * (k1 * row_scale[nt][e]) : kNegInf;
-          m_new[nt][e] = fmax3(m_new[nt][e], x, y);
+          s[mt][nt][e] *= k0 * row_scale[nt][e];
+          s[mt][nt][2 + e] *= k1 * row_scale[nt][e];
         }
+      if (!plain) {
+        const int r = mt * 16 + token_of(g);
+        const bool in0 = r < left && __float_as_uint(k0) != kNoPage, in1 = r + 8 < left && __float_as_uint(k1) != kNoPage;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            s[mt][nt][e] = in0 ? s[mt][nt][e] : kNegInf;
+            s[mt][nt][2 + e] = in1 ? s[mt][nt][2 + e] : kNegInf;
+          }
+      }
     }
-#pragma unroll
-    for (int x = 4; x < 32; x <<= 1)
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) m_new[nt][e] = fmaxf(m_new[nt][e], __shfl_xor_sync(0xffffffffu, m_new[nt][e], x));
-    // ---- The products with V take p * vs relative to the largest |vs| so far (its power of two), so that they are fp16
-    // numbers near 1 whatever the pages' scales: rounding them costs 2^-11 of each, 2^-25 of the unit when they are tiny.
-    v_top = min(__reduce_max_sync(0xffffffffu, v_top) & 0x7f800000u, 0x7e800000u);
-    const float vref_new = fmaxf(vref, __uint_as_float(v_top));
-    const float v_inv = __uint_as_float((254u << 23) - __float_as_uint(vref_new));
-    bool moved = vref_new != vref;
-    float alpha[NT][2];
-    const float v_alpha = vref * v_inv;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        moved = moved || m_new[nt][e] != m[nt][e];
-        m[nt][e] = m[nt][e] == m_new[nt][e] ? 0.f : m[nt][e] - m_new[nt][e];
-        alpha[nt][e] = fast_exp2(m[nt][e]);
-        m[nt][e] = m_new[nt][e];
-        l[nt][e] *= alpha[nt][e];
+        float top = kNegInf;
+#pragma unroll
+        for (int mt = 0; mt < kMt; ++mt) top = fmax3(top, s[mt][nt][e], s[mt][nt][2 + e]);
+        excess = fmaxf(excess, top - m[nt][e]);  // (-inf) - (-inf) is NaN, which loses
       }
-    if (__any_sync(0xffffffffu, moved)) {
+    if (__any_sync(0xffffffffu, excess > kSlack || v_moves)) {
+      uint32_t v_top = 0u;
+#pragma unroll
+      for (int mt = 0; mt < kMt; ++mt)
+        v_top = max(v_top, max(__float_as_uint(v_scale[mt][0]) & 0x7fffffffu, __float_as_uint(v_scale[mt][1]) & 0x7fffffffu));
+      v_top = min(__reduce_max_sync(0xffffffffu, v_top) & 0x7f800000u, 0x7e800000u);
+      const float vref_new = fmaxf(vref, __uint_as_float(v_top));
+      const float v_alpha = vref * __uint_as_float((254u << 23) - __float_as_uint(vref_new));
+      vref = vref_new;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const float f0 = alpha[nt][0] * v_alpha, f1 = alpha[nt][1] * v_alpha;
+        float f[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float top = m[nt][e];
+#pragma unroll
+          for (int mt = 0; mt < kMt; ++mt) top = fmax3(top, s[mt][nt][e], s[mt][nt][2 + e]);
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+          const float alpha = top == m[nt][e] ? 1.f : fast_exp2(m[nt][e] - top);
+          m[nt][e] = top;
+          l[nt][e] *= alpha;
+          f[e] = alpha * v_alpha;
+        }
 #pragma unroll
         for (int i = 0; i < kNm; ++i) {
-          o[nt][i][0] *= f0;
-          o[nt][i][1] *= f1;
-          o[nt][i][2] *= f0;
-          o[nt][i][3] *= f1;
+          o[nt][i][0] *= f[0];
+          o[nt][i][1] *= f[1];
+          o[nt][i][2] *= f[0];
+          o[nt][i][3] *= f[1];
         }
       }
     }
-    vref = vref_new;
+    const float v_inv = __uint_as_float((254u << 23) - __float_as_uint(vref));
     // ---- probabilities and the products with V: rows are dimensions, columns query heads
 #pragma unroll
     for (int mt = 0; mt < kMt; ++mt) {
@@ -472,7 +567,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_kernel(const Args a) {
         b0[nt] = transpose8x8(DType<__half>::pack2(p00 * v0, p01 * v0));
         b1[nt] = transpose8x8(DType<__half>::pack2(p10 * v1, p11 * v1));
       }
-      const int ra = mt * 16 + token_of(2 * t4), rb = mt * 16 + token_of(2 * t4 + 1);
       auto product = [&](int i, uint32_t wa, uint32_t wb, uint32_t wc, uint32_t wd) {
         // four dimensions of tokens ra, rb (and ra + 8, rb + 8): tiles i (dimensions 0, 1) and i + 1 (2, 3)
         const uint32_t x = __byte_perm(wa, wb, 0x5140), y = __byte_perm(wc, wd, 0x5140);
@@ -485,17 +579,33 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_kernel(const Args a) {
           mma(o[nt][i + 1], c0, c1, c2, c3, b0[nt], b1[nt]);
         }
       };
+      // rows behind the context may hold anything, NaN among it: zeros there
+      const int r = mt * 16 + token_of(2 * t4), r2 = mt * 16 + token_of(2 * t4 + 1);
+      const uint32_t row_a = vt + mt * step16 + va_row, row_b = vt + mt * step16 + vb_row;
       if constexpr (D == 64) {
-        const int at = (g & 1) * 8;
-        const uint2 va = lds64(vt + chunk_at<D>(ra, g >> 1) + at), vb = lds64(vt + chunk_at<D>(rb, g >> 1) + at);
-        const uint2 vc = lds64(vt + chunk_at<D>(ra + 8, g >> 1) + at), vd = lds64(vt + chunk_at<D>(rb + 8, g >> 1) + at);
+        const uint32_t ca = ((uint32_t)((g >> 1) << 4) ^ va_swz) + (g & 1) * 8, cb = ((uint32_t)((g >> 1) << 4) ^ vb_swz) + (g & 1) * 8;
+        uint2 va = lds64(row_a + ca), vb = lds64(row_b + cb);
+        uint2 vc = lds64(row_a + step8 + ca), vd = lds64(row_b + step8 + cb);
+        if (!plain) {
+          if (r >= left) va = make_uint2(0u, 0u);
+          if (r2 >= left) vb = make_uint2(0u, 0u);
+          if (r + 8 >= left) vc = make_uint2(0u, 0u);
+          if (r2 + 8 >= left) vd = make_uint2(0u, 0u);
+        }
         product(0, va.x, vb.x, vc.x, vd.x);
         product(2, va.y, vb.y, vc.y, vd.y);
       } else {
 #pragma unroll
         for (int h = 0; h < D / 128; ++h) {
-          const uint4 va = lds128(vt + chunk_at<D>(ra, g + 8 * h)), vb = lds128(vt + chunk_at<D>(rb, g + 8 * h));
-          const uint4 vc = lds128(vt + chunk_at<D>(ra + 8, g + 8 * h)), vd = lds128(vt + chunk_at<D>(rb + 8, g + 8 * h));
+          const uint32_t ca = ((uint32_t)(g << 4) ^ va_swz) + h * kHalfBytes, cb = ((uint32_t)(g << 4) ^ vb_swz) + h * kHalfBytes;
+          uint4 va = lds128(row_a + ca), vb = lds128(row_b + cb);
+          uint4 vc = lds128(row_a + step8 + ca), vd = lds128(row_b + step8 + cb);
+          if (!plain) {
+            if (r >= left) va = make_uint4(0u, 0u, 0u, 0u);
+            if (r2 >= left) vb = make_uint4(0u, 0u, 0u, 0u);
+            if (r + 8 >= left) vc = make_uint4(0u, 0u, 0u, 0u);
+            if (r2 + 8 >= left) vd = make_uint4(0u, 0u, 0u, 0u);
+          }
           product(8 * h, va.x, vb.x, vc.x, vd.x);
           product(8 * h + 2, va.y, vb.y, vc.y, vd.y);
           product(8 * h + 4, va.z, vb.z, vc.z, vd.z);
@@ -503,11 +613,16 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_kernel(const Args a) {
         }
       }
     }
-    stage = stage + 1 == kStages ? 0 : stage + 1;
+    __syncwarp();  // every lane is done with the stage
+    if (lane == 0) mbar_arrive(&empty_s[stage]);
+    if (++stage == kStages) {
+      stage = 0;
+      parity ^= 1;
+    }
 
     // ---- the item ends here, or this CTA's part of it does
-    if (get.step + 1 == get.steps || u + 1 == units) {
-      const bool whole = begin_step == 0 && get.step + 1 == get.steps;
+    if (at.step + 1 == at.steps || u + 1 == units) {
+      const bool whole = begin_step == 0 && at.step + 1 == at.steps;
       const int slot = blockIdx.x * 2 + (begin_step > 0 ? 0 : 1);
       const int rows = item_rows(heads_cta, NT);
       float weight[NT][2], top[NT][2], sum[NT][2];
@@ -521,23 +636,23 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_kernel(const Args a) {
           sum[nt][e] = l[nt][e];
           weight[nt][e] = vref;
         }
-      if (a.warps_per_head > 1) {  // the warps of a head took its tokens by turns
+      if (warps_head > 1) {  // the warps of a head took its tokens by turns
         if (g == 0)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e)
-              stats[warp * kRows + nt * 8 + 2 * t4 + e] = make_float4(m[nt][e], l[nt][e], 0.f, 0.f);
-        head_barrier(1 + wh, a.warps_per_head * 32);
+              stats[warp * kRows + nt * 8 + 2 * t4 + e] = make_float2(m[nt][e], l[nt][e]);
+        head_barrier(1 + wh, warps_head * 32);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             float M = kNegInf, L = 0.f;
-            const float4* at = stats + (warp - wt) * kRows + nt * 8 + 2 * t4 + e;
-            for (int w = 0; w < a.warps_per_head; ++w) M = fmaxf(M, at[w * kRows].x);
+            const float2* peer = stats + (warp - wt) * kRows + nt * 8 + 2 * t4 + e;
+            for (int w = 0; w < warps_head; ++w) M = fmaxf(M, peer[w * kRows].x);
             const float z = M == kNegInf ? 0.f : M;
-            for (int w = 0; w < a.warps_per_head; ++w) L += at[w * kRows].y * fast_exp2(at[w * kRows].x - z);
+            for (int w = 0; w < warps_head; ++w) L += peer[w * kRows].y * fast_exp2(peer[w * kRows].x - z);
             weight[nt][e] = vref * fast_exp2(m[nt][e] - z);
             top[nt][e] = M;
             sum[nt][e] = L;
@@ -559,7 +674,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_kernel(const Args a) {
       auto put4 = [&](int row, int d, float4 x) {
         if (chunk0 + row >= a.group || d >= a.head_dim) return;
         if (whole) {
-          uint16_t* to = static_cast<uint16_t*>(a.out) + get.b * a.o_sb + (int64_t)(head * a.group + chunk0 + row) * a.o_sh + d;
+          uint16_t* to = static_cast<uint16_t*>(a.out) + at.b * a.o_sb + (int64_t)(head * a.group + chunk0 + row) * a.o_sh + d;
           *reinterpret_cast<uint2*>(to) = a.dtype == FA_F16
               ? make_uint2(DType<__half>::pack2(x.x, x.y), DType<__half>::pack2(x.z, x.w))
               : make_uint2(DType<__nv_bfloat16>::pack2(x.x, x.y), DType<__nv_bfloat16>::pack2(x.z, x.w));
@@ -568,7 +683,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_kernel(const Args a) {
         }
       };
       constexpr int kPerLane = D == 64 ? 8 : 16;  // neighbouring dimensions of a lane group g
-      if (a.warps_per_head == 1) {
+      if (warps_head == 1) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -592,12 +707,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_kernel(const Args a) {
                 *reinterpret_cast<float2*>(mine + (nt * 8 + 2 * t4 + e) * kCols + g * 2 * kRoundTiles + 2 * i) =
                     make_float2(x[e] * weight[nt][e], x[2 + e] * weight[nt][e]);
               }
-          head_barrier(1 + wh, a.warps_per_head * 32);
-          for (int x = wt * 32 + lane; x < 128; x += a.warps_per_head * 32) {
+          head_barrier(1 + wh, warps_head * 32);
+          for (int x = wt * 32 + lane; x < 128; x += warps_head * 32) {
             const int row = x * 4 / kCols, col = x * 4 % kCols;
             const float* from = merge + (warp - wt) * 512 + x * 4;
             float4 acc = *reinterpret_cast<const float4*>(from);
-            for (int w = 1; w < a.warps_per_head; ++w) {
+            for (int w = 1; w < warps_head; ++w) {
               const float4 y = *reinterpret_cast<const float4*>(from + w * 512);
               acc.x += y.x;
               acc.y += y.y;
@@ -607,117 +722,111 @@ __global__ void __launch_bounds__(kThreads, 1) paged8_kernel(const Args a) {
             const int tile = round * kRoundTiles + (col % (2 * kRoundTiles)) / 2;
             put4(row, (tile / 8) * 128 + kPerLane * (col / (2 * kRoundTiles)) + 2 * (tile % 8), acc);
           }
-          head_barrier(1 + wh, a.warps_per_head * 32);
+          head_barrier(1 + wh, warps_head * 32);
         }
       }
     }
-    if (u + 1 < units) get.advance(a, span, items);
-    __syncwarp();  // every lane is done with the stage before it is filled again
+    if (u + 1 < units) at.advance(a, span, items);
   }
 }
 
-// Joins the parts of the items that several CTAs share. The boundary between the stretches of CTAs i - 1 and i lies inside
-// at most one item; an item of `parts` stretches has parts - 1 boundaries, and their blocks share its rows.
+// Joins the parts of the items that several CTAs share. A stretch that begins inside an item is one cut of it; an item of
+// `parts` stretches has parts - 1 cuts, whose blocks (kMergeSplit a cut) share its rows. With few parts a warp takes a row,
+// all of whose parts it loads at once; with many a block does.
+constexpr int kMergeSplit = 4;
 template <int D, int NT>
-__global__ void __launch_bounds__(kThreads) paged8_merge_kernel(const Args a, int grid_ctas) {
+__global__ void __launch_bounds__(kMergeThreads) paged8_merge_kernel(const Args a) {
+  constexpr int kVec = (D + 127) / 128;
   __shared__ float weight_s[kMaxCtas];
-  __shared__ float red_s[kWarps][D];
-  __shared__ float part_s[kWarps];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  __shared__ float red_s[kMergeThreads / 32][D];
+  __shared__ float part_s[kMergeThreads / 32];
+  grid_dependency_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int64_t total = a.prefix[a.batch];
-  const int64_t ctas = min((int64_t)grid_ctas, total);
-  const int boundary = blockIdx.x + 1;
-  if (boundary >= ctas) return;
-  const int64_t u = boundary * total / ctas;
-  int lo = 0, hi = a.batch - 1;  // the last request that starts at or before u (requests without units start there too)
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (a.prefix[mid] <= u) lo = mid;
-    else hi = mid - 1;
-  }
-  const int b = lo, items = a.head_ctas * a.row_chunks;
-  const int64_t first = a.prefix[b], steps = (a.prefix[b + 1] - first) / items;
-  const int item = (int)((u - first) / steps);
-  const int64_t begin = first + item * steps;
-  if (begin == u) return;
-  const int c0 = (int)(((begin + 1) * ctas - 1) / total), c1 = (int)(((begin + steps) * ctas - 1) / total);
-  const int parts = c1 - c0 + 1, share = parts - 1;
-  const int heads_cta = kWarps / a.warps_per_head, rows = item_rows(heads_cta, NT);
-  const int head0 = (item / a.row_chunks) * heads_cta, chunk0 = (item % a.row_chunks) * NT * 8;
-  auto part_row = [&](int p, int row) { return ((int64_t)(2 * (c0 + p) + (p == 0 ? 1 : 0)) * rows + row); };
+  const int4 cut = a.cuts[blockIdx.x + 1];
+  const int b = cut.x, item = cut.y, c0 = cut.z, parts = cut.w;
+  if (parts == 0) return;
+  const int head0 = (item / a.row_chunks) << a.head_shift, chunk0 = (item % a.row_chunks) * NT * 8;
+  const int slots = item_rows(1 << a.head_shift, NT);               // rows of a part in the workspace
+  const int live = min(NT * 8, a.group - chunk0), rows = live << a.head_shift;  // query heads there are
+  const int turn = ((int)blockIdx.x - c0) * kMergeSplit + blockIdx.y, share = (parts - 1) * kMergeSplit;
+  auto part_row = [&](int p, int row) {
+    return (int64_t)(2 * (c0 + p) + (p == 0 ? 1 : 0)) * slots + (row / live) * NT * 8 + row % live;
+  };
   auto store4 = [&](int row, int d, float4 x) {
-    uint16_t* to = static_cast<uint16_t*>(a.out) + b * a.o_sb +
-                   (int64_t)((head0 + row / (NT * 8)) * a.group + chunk0 + row % (NT * 8)) * a.o_sh + d;
+    uint16_t* to = static_cast<uint16_t*>(a.out) + b * a.o_sb + (int64_t)((head0 + row / live) * a.group + chunk0 + row % live) * a.o_sh + d;
     *reinterpret_cast<uint2*>(to) = a.dtype == FA_F16
         ? make_uint2(DType<__half>::pack2(x.x, x.y), DType<__half>::pack2(x.z, x.w))
         : make_uint2(DType<__nv_bfloat16>::pack2(x.x, x.y), DType<__nv_bfloat16>::pack2(x.z, x.w));
   };
-  auto is_row = [&](int row) { return row < rows && chunk0 + row % (NT * 8) < a.group; };
-  const int turn = boundary - c0 - 1;
 
-  if (parts <= 8) {  // few parts: a warp takes a row
-    for (int row = turn + share * warp; row < rows; row += share * kWarps) {
-      if (!is_row(row)) continue;
+  if (parts <= 8) {
+    for (int row = turn + share * warp; row < rows; row += share * (kMergeThreads / 32)) {
+      float4 x[8][kVec];
+#pragma unroll
+      for (int p = 0; p < 8; ++p)
+#pragma unroll
+        for (int c = 0; c < kVec; ++c) {
+          x[p][c] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (p < parts && lane * 4 + c * 128 < a.head_dim)
+            x[p][c] = *reinterpret_cast<const float4*>(a.part_o + part_row(p, row) * D + lane * 4 + c * 128);
+        }
       float2 st = make_float2(kNegInf, 0.f);
       if (lane < parts) st = *reinterpret_cast<const float2*>(a.part_stat + part_row(lane, row) * 2);
       float top = st.x;
 #pragma unroll
-      for (int x = 4; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+      for (int i = 4; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
       float w = fast_exp2(st.x - (top == kNegInf ? 0.f : top)), sum = w * st.y;
 #pragma unroll
-      for (int x = 4; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+      for (int i = 4; i > 0; i >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, i);
       w = sum == 0.f ? 0.f : w / sum;
-      float4 acc[(D + 127) / 128];
+      float4 acc[kVec];
 #pragma unroll
-      for (int c = 0; c < (D + 127) / 128; ++c) acc[c] = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int p = 0; p < parts; ++p) {
+      for (int c = 0; c < kVec; ++c) acc[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int p = 0; p < 8; ++p) {
         const float f = __shfl_sync(0xffffffffu, w, p);  // lanes 0 .. 7 hold the parts' weights
+        if (p >= parts) continue;
 #pragma unroll
-        for (int c = 0; c < (D + 127) / 128; ++c) {
-          const int d = lane * 4 + c * 128;
-          if (d >= a.head_dim) continue;
-          const float4 x = *reinterpret_cast<const float4*>(a.part_o + part_row(p, row) * D + d);
-          acc[c].x += f * x.x;
-          acc[c].y += f * x.y;
-          acc[c].z += f * x.z;
-          acc[c].w += f * x.w;
+        for (int c = 0; c < kVec; ++c) {
+          acc[c].x += f * x[p][c].x;
+          acc[c].y += f * x[p][c].y;
+          acc[c].z += f * x[p][c].z;
+          acc[c].w += f * x[p][c].w;
         }
       }
 #pragma unroll
-      for (int c = 0; c < (D + 127) / 128; ++c)
+      for (int c = 0; c < kVec; ++c)
         if (lane * 4 + c * 128 < a.head_dim) store4(row, lane * 4 + c * 128, acc[c]);
     }
     return;
   }
-  for (int row = turn; row < rows; row += share) {  // many parts: the block takes a row
-    if (!is_row(row)) continue;
-    float2 st = make_float2(kNegInf, 0.f);
-    if (tid < parts) st = *reinterpret_cast<const float2*>(a.part_stat + part_row(tid, row) * 2);
+  for (int row = turn; row < rows; row += share) {
+    const float2 st = tid < parts ? *reinterpret_cast<const float2*>(a.part_stat + part_row(tid, row) * 2)
+                                  : make_float2(kNegInf, 0.f);
     float top = st.x;
 #pragma unroll
-    for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+    for (int i = 16; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
     __syncthreads();
     if (lane == 0) part_s[warp] = top;
     __syncthreads();
-    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, part_s[w]);
+    for (int w = 0; w < kMergeThreads / 32; ++w) top = fmaxf(top, part_s[w]);
     const float w = fast_exp2(st.x - (top == kNegInf ? 0.f : top));
     float sum = w * st.y;
     weight_s[tid] = w;
 #pragma unroll
-    for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+    for (int i = 16; i > 0; i >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, i);
     __syncthreads();
     if (lane == 0) part_s[warp] = sum;
     __syncthreads();
     sum = 0.f;
-    for (int i = 0; i < kWarps; ++i) sum += part_s[i];
+    for (int i = 0; i < kMergeThreads / 32; ++i) sum += part_s[i];
     const float inverse = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
     for (int d = lane * 4; d < D; d += 128) {
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
       if (d < a.head_dim) {
-#pragma unroll 4
-        for (int p = warp; p < parts; p += kWarps) {
+#pragma unroll 8
+        for (int p = warp; p < parts; p += kMergeThreads / 32) {
           const float f = weight_s[p];
           const float4 x = *reinterpret_cast<const float4*>(a.part_o + part_row(p, row) * D + d);
           acc.x += f * x.x;
@@ -731,7 +840,7 @@ __global__ void __launch_bounds__(kThreads) paged8_merge_kernel(const Args a, in
     __syncthreads();
     if (tid * 4 < a.head_dim) {
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int i = 0; i < kWarps; ++i) {
+      for (int i = 0; i < kMergeThreads / 32; ++i) {
         const float4 x = *reinterpret_cast<const float4*>(&red_s[i][tid * 4]);
         acc.x += x.x;
         acc.y += x.y;
@@ -745,16 +854,19 @@ __global__ void __launch_bounds__(kThreads) paged8_merge_kernel(const Args a, in
 
 // How a head layout is cut: padded head dim, query heads an item takes (8 or 16), kv heads a CTA takes.
 struct Shape {
-  int D, nt, heads_cta, row_chunks;
+  int D, nt, head_shift, row_chunks, box_shift;
 };
-Shape shape_of(int head_dim, int heads_q, int heads_kv) {
+Shape shape_of(const fa_paged8_params& p) {
   Shape s;
-  s.D = head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256;
-  const int group = heads_q / heads_kv;
+  const int group = p.heads_q / p.heads_kv;
+  s.head_shift = 3;
+  while (p.heads_kv % (1 << s.head_shift)) --s.head_shift;
+  s.box_shift = 0;
+  while (s.box_shift < 4 && (2 << s.box_shift) <= p.block_size) ++s.box_shift;
+  // (a box of one 64-byte row would not start on the 128 bytes that TMA asks for: such rows are padded to 128)
+  s.D = p.head_dim <= 64 && s.head_shift + s.box_shift > 0 ? 64 : p.head_dim <= 128 ? 128 : 256;
   s.nt = group > 8 && s.D <= 128 ? 2 : 1;
   s.row_chunks = (group + s.nt * 8 - 1) / (s.nt * 8);
-  s.heads_cta = 8;
-  while (heads_kv % s.heads_cta) s.heads_cta /= 2;
   return s;
 }
 
@@ -768,16 +880,30 @@ int cta_count() {
   return sms < kMaxCtas ? sms : kMaxCtas;
 }
 
-int64_t prefix_bytes(int batch) { return ((int64_t)(batch + 1) * 8 + 15) / 16 * 16; }
+// (dim, token of the page, head, page) with a box of one row's bytes x a box's tokens x a CTA's heads
+int make_cache_map(CUtensorMap* map, const void* ptr, const fa_paged8_params& p, const int64_t (&st)[4], const Shape& s) {
+  TensorMapEncodeFn enc = tensor_map_encoder();
+  if (enc == nullptr) return set_error(FA_ERR_DEVICE, "cuTensorMapEncodeTiled is not available from this driver");
+  const cuuint64_t dims[4] = {(cuuint64_t)p.head_dim, (cuuint64_t)p.block_size, (cuuint64_t)p.heads_kv, (cuuint64_t)p.num_blocks};
+  auto stride = [&](int64_t x, int64_t n) { return (cuuint64_t)(n > 1 ? x : 256); };  // a size-1 dimension never advances
+  const cuuint64_t strides[3] = {stride(st[1], p.block_size), stride(st[2], p.heads_kv), stride(st[0], p.num_blocks)};
+  const cuuint32_t box[4] = {(cuuint32_t)(s.D < 128 ? s.D : 128), 1u << s.box_shift, 1u << s.head_shift, 1};
+  const cuuint32_t one[4] = {1, 1, 1, 1};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(ptr), dims, strides, box, one,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, s.D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(FA_ERR_UNSUPPORTED, "8-bit paged decode: no tensor map for this cache layout (code %d)", (int)r);
+  return 0;
+}
 
 template <typename C8, int D, int NT>
-int launch(const Args& a, int ctas, cudaStream_t stream) {
+int launch(const CUtensorMap& k, const CUtensorMap& v, const Args& a, int ctas, cudaStream_t stream) {
   auto kernel = paged8_kernel<C8, D, NT>;
   constexpr int smem = Smem<D, NT>::kBytes;
-  static_assert(smem <= 227 * 1024 - 256, "shared memory of an SM");
+  static_assert(smem <= 227 * 1024 - 512, "shared memory of an SM");
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e == cudaSuccess) {
-    kernel<<<ctas, kThreads, smem, stream>>>(a);
+    kernel<<<ctas, kThreads, smem, stream>>>(k, v, a);
     e = cudaGetLastError();
   }
   if (e == cudaSuccess && ctas > 1) {
@@ -785,12 +911,12 @@ int launch(const Args& a, int ctas, cudaStream_t stream) {
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(ctas - 1);
-    cfg.blockDim = dim3(kThreads);
+    cfg.gridDim = dim3(ctas - 1, kMergeSplit);
+    cfg.blockDim = dim3(kMergeThreads);
     cfg.stream = stream;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, paged8_merge_kernel<D, NT>, a, ctas);
+    e = cudaLaunchKernelEx(&cfg, paged8_merge_kernel<D, NT>, a);
   }
   if (e == cudaSuccess) return 0;
   cudaGetLastError();
@@ -798,10 +924,10 @@ int launch(const Args& a, int ctas, cudaStream_t stream) {
 }
 
 template <typename C8>
-int dispatch(const Shape& s, const Args& a, int ctas, cudaStream_t stream) {
-  if (s.D == 64) return s.nt == 1 ? launch<C8, 64, 1>(a, ctas, stream) : launch<C8, 64, 2>(a, ctas, stream);
-  if (s.D == 128) return s.nt == 1 ? launch<C8, 128, 1>(a, ctas, stream) : launch<C8, 128, 2>(a, ctas, stream);
-  return launch<C8, 256, 1>(a, ctas, stream);
+int dispatch(const Shape& s, const CUtensorMap& k, const CUtensorMap& v, const Args& a, int ctas, cudaStream_t stream) {
+  if (s.D == 64) return s.nt == 1 ? launch<C8, 64, 1>(k, v, a, ctas, stream) : launch<C8, 64, 2>(k, v, a, ctas, stream);
+  if (s.D == 128) return s.nt == 1 ? launch<C8, 128, 1>(k, v, a, ctas, stream) : launch<C8, 128, 2>(k, v, a, ctas, stream);
+  return launch<C8, 256, 1>(k, v, a, ctas, stream);
 }
 
 }  // namespace
@@ -809,43 +935,37 @@ int dispatch(const Shape& s, const Args& a, int ctas, cudaStream_t stream) {
 int64_t paged8_workspace_bytes(const fa_paged8_params& p) {
   const int ctas = cta_count();
   if (ctas < 0) return ctas;
-  const Shape s = shape_of(p.head_dim, p.heads_q, p.heads_kv);
-  return prefix_bytes(p.batch) + (int64_t)2 * ctas * item_rows(s.heads_cta, s.nt) * (s.D + 2) * 4;
+  const Shape s = shape_of(p);
+  return (int64_t)ctas * sizeof(int4) + (int64_t)2 * ctas * item_rows(1 << s.head_shift, s.nt) * (s.D + 2) * 4;
 }
 
 int launch_decode_paged8(const fa_paged8_params& p, cudaStream_t stream) {
   const int ctas = cta_count();
   if (ctas < 0) return ctas;
-  const Shape s = shape_of(p.head_dim, p.heads_q, p.heads_kv);
-  for (int i = 0; i < 2; ++i)
-    if ((uint64_t)p.k_strides[i] > UINT32_MAX || (uint64_t)p.v_strides[i] > UINT32_MAX)
-      return set_error(FA_ERR_UNSUPPORTED, "8-bit paged decode: block and token strides must be below 2^32");
+  const Shape s = shape_of(p);
   if (((int64_t)p.max_blocks * p.block_size) > INT32_MAX)
     return set_error(FA_ERR_UNSUPPORTED, "8-bit paged decode: a block table of more than 2^31 - 1 tokens");
+  CUtensorMap k, v;
+  int rc = make_cache_map(&k, p.k_cache, p, p.k_strides, s);
+  if (!rc) rc = make_cache_map(&v, p.v_cache, p, p.v_strides, s);
+  if (rc) return rc;
   Args a = {};
   a.dtype = p.dtype;
   a.batch = p.batch;
   a.heads_q = p.heads_q;
-  a.heads_kv = p.heads_kv;
   a.head_dim = p.head_dim;
   a.group = p.heads_q / p.heads_kv;
   a.num_blocks = p.num_blocks;
   a.max_blocks = p.max_blocks;
   while ((1 << a.shift) < p.block_size) ++a.shift;
-  a.head_ctas = p.heads_kv / s.heads_cta;
+  a.head_shift = s.head_shift;
+  a.head_ctas = p.heads_kv >> s.head_shift;
   a.row_chunks = s.row_chunks;
-  a.warps_per_head = kWarps / s.heads_cta;
+  a.box_shift = s.box_shift;
+  a.scale_shift = s.box_shift < 3 ? s.box_shift : 3;
   a.q = p.q;
   a.q_sb = p.q_strides[0];
   a.q_sh = p.q_strides[1];
-  a.k = static_cast<const uint8_t*>(p.k_cache);
-  a.v = static_cast<const uint8_t*>(p.v_cache);
-  a.k_sb = (uint32_t)p.k_strides[0];
-  a.k_st = (uint32_t)p.k_strides[1];
-  a.k_sh = p.k_strides[2];
-  a.v_sb = (uint32_t)p.v_strides[0];
-  a.v_st = (uint32_t)p.v_strides[1];
-  a.v_sh = p.v_strides[2];
   a.ks = p.k_scales;
   a.vs = p.v_scales;
   a.ks_sb = p.ks_strides[0];
@@ -861,12 +981,12 @@ int launch_decode_paged8(const fa_paged8_params& p, cudaStream_t stream) {
   a.o_sb = p.o_strides[0];
   a.o_sh = p.o_strides[1];
   a.scale_log2 = p.softmax_scale * kLog2e;
-  uint8_t* ws = static_cast<uint8_t*>(p.workspace);
-  a.prefix = reinterpret_cast<int64_t*>(ws);
-  a.part_stat = reinterpret_cast<float*>(ws + prefix_bytes(p.batch));
-  a.part_o = a.part_stat + (int64_t)2 * ctas * item_rows(s.heads_cta, s.nt) * 2;
-  return p.cache_dtype == FA_CACHE_E4M3 ? dispatch<CodeE4M3>(s, a, ctas, stream)
-                                        : dispatch<CodeInt8>(s, a, ctas, stream);
+  a.status = p.status;
+  a.cuts = static_cast<int4*>(p.workspace);
+  a.part_stat = reinterpret_cast<float*>(a.cuts + ctas);
+  a.part_o = a.part_stat + (int64_t)2 * ctas * item_rows(1 << s.head_shift, s.nt) * 2;
+  return p.cache_dtype == FA_CACHE_E4M3 ? dispatch<CodeE4M3>(s, k, v, a, ctas, stream)
+                                        : dispatch<CodeInt8>(s, k, v, a, ctas, stream);
 }
 
 }  // namespace fa

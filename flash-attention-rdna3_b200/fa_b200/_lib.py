@@ -9,6 +9,7 @@ import threading
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libfa_b200.so")
+BINDING_PATH = os.path.join(_HERE, "_paged_native.so")
 
 FA_F16, FA_BF16, FA_F32 = 0, 1, 2
 FA_PATH_NONE, FA_PATH_TCGEN05, FA_PATH_SIMT = 0, 1, 2
@@ -170,7 +171,7 @@ class Paged8Params(C.Structure):
         ("context_lens", C.c_void_p), ("cl_stride", C.c_int64),
         ("out", C.c_void_p), ("o_strides", I64x3),
         ("softmax_scale", C.c_float),
-        ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64), ("status", C.c_void_p),
     ]
 
 
@@ -224,6 +225,32 @@ def load():
                                    f"{ABI_VERSION}; rebuild it with `python flash-attention-rdna3_b200/build.py`")
             _lib = lib
     return _lib
+
+
+_binding = None
+
+
+def paged_binding():
+    """The compiled binding of the paged-cache calls (csrc/fa_paged8_bind.cpp), bound to the loaded library."""
+    global _binding
+    if _binding is not None:
+        return _binding
+    lib = load()
+    with _lock:
+        if _binding is None:
+            if not os.path.exists(BINDING_PATH):
+                raise RuntimeError(
+                    f"fa_b200: {BINDING_PATH} is missing; build it with "
+                    "`python flash-attention-rdna3_b200/build.py` (there is no fallback path)")
+            import importlib.util
+
+            spec = importlib.util.spec_from_file_location("_paged_native", BINDING_PATH)
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+            module.bind(*(C.cast(getattr(lib, name), C.c_void_p).value for name in (
+                "fa_paged_plan", "fa_paged8_append", "fa_decode_paged8", "fa_workspace_bytes", "fa_last_error_string")))
+            _binding = module
+    return _binding
 
 
 def check(rc):

@@ -8,6 +8,9 @@ rest of a server's step; these are the operators around `flash_attention_decode_
   flash_attention_decode_paged_8bit   one query token for each request against the cache
   PagedKVCache8                       a cache of several layers that runs the three together
 
+Each function first offers its arguments to the compiled binding (csrc/fa_paged8_bind.cpp), which launches at once or
+declines; what it declines - refusals, copies, traced tensors - is handled here.
+
 Caches are ``(num_blocks, block_size, kv_heads, head_dim)`` in ``torch.float8_e4m3fn`` or ``torch.int8`` with fp32 scales
 ``(num_blocks, kv_heads)``: a code c of block p and head h stands for ``c * scales[p, h]``.
 """
@@ -107,6 +110,11 @@ def paged_kv_plan(context_lens, new_lens, block_table, free_blocks, free_count, 
     the packed batch (as ``flash_attention_varlen`` takes them); the lengths after the step (0 for ended requests) and
     the pages then left. The last two are new tensors, or with ``inplace=True`` the given ones, overwritten.
     """
+    if not torch.compiler.is_compiling():
+        planned = _lib.paged_binding().plan(context_lens, new_lens, block_table, free_blocks, free_count, num_tokens,
+                                            block_size, bool(inplace))
+        if planned is not None:
+            return planned
     validate_paged_plan_inputs(context_lens, new_lens, block_table, free_blocks, free_count, num_tokens, block_size,
                                inplace)
     num_tokens, block_size = int(num_tokens), int(block_size)
@@ -136,6 +144,7 @@ def _append_impl(key, value, k_cache, v_cache, k_scales, v_scales, slot_mapping)
         k_scales.stride(), v_scales.data_ptr(), v_scales.stride(), slot_mapping.data_ptr(), slot_mapping.stride(0),
         _status_word(device).data_ptr())
     _call(lib.fa_paged8_append, p, device)
+    _lib.paged_binding().set_status(device.index, p.status)
 
 
 @torch.library.custom_op("fa_b200::paged_kv_append", mutates_args=("k_cache", "v_cache", "k_scales", "v_scales"))
@@ -162,6 +171,9 @@ def paged_kv_append(key, value, k_cache, v_cache, k_scales, v_scales, slot_mappi
     The new tokens of a page have to be neighbours in ``slot_mapping`` with slots that rise by one, and a page belongs to
     one request; `check_status` raises after a call that repeats a slot or goes back inside a page. Inference-only.
     """
+    if not torch.compiler.is_compiling() and _lib.paged_binding().append(key, value, k_cache, v_cache, k_scales, v_scales,
+                                                                         slot_mapping):
+        return
     validate_paged8_append_inputs(key, value, k_cache, v_cache, k_scales, v_scales, slot_mapping)
     validate_inference_only(key, value)
     if _direct(key):
@@ -174,8 +186,8 @@ def paged_kv_append(key, value, k_cache, v_cache, k_scales, v_scales, slot_mappi
 # decode
 # ---------------------------------------------------------------------------------------------------
 @functools.lru_cache(maxsize=4096)
-def _workspace_bytes(device_index, batch, heads_q, heads_kv, head_dim):
-    p = _lib.Paged8Params(batch=batch, heads_q=heads_q, heads_kv=heads_kv, head_dim=head_dim)
+def _workspace_bytes(device_index, batch, heads_q, heads_kv, head_dim, block_size):
+    p = _lib.Paged8Params(batch=batch, heads_q=heads_q, heads_kv=heads_kv, head_dim=head_dim, block_size=block_size)
     with torch.cuda.device(device_index):
         n = _lib.load().fa_workspace_bytes(_lib.FA_WS_PAGED8, C.byref(p))
     if n < 0:
@@ -190,15 +202,17 @@ def _decode8_impl(query, k_cache, v_cache, k_scales, v_scales, block_table, cont
     blocks, block_size, heads_kv, _ = k_cache.shape
     query = query if _vector_friendly(query) else query.contiguous()
     out = torch.empty((batch, heads_q, head_dim), dtype=query.dtype, device=device)
-    nbytes = _workspace_bytes(device.index, batch, heads_q, heads_kv, head_dim)
+    nbytes = _workspace_bytes(device.index, batch, heads_q, heads_kv, head_dim, block_size)
     workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
     p = _lib.Paged8Params(
         _DTYPE_CODE[query.dtype], _CACHE_CODE[k_cache.dtype], batch, heads_q, heads_kv, head_dim, blocks, block_size,
         block_table.shape[1], query.data_ptr(), query.stride(), k_cache.data_ptr(), k_cache.stride(),
         v_cache.data_ptr(), v_cache.stride(), k_scales.data_ptr(), k_scales.stride(), v_scales.data_ptr(),
         v_scales.stride(), block_table.data_ptr(), block_table.stride(), context_lens.data_ptr(),
-        context_lens.stride(0), out.data_ptr(), out.stride(), softmax_scale, workspace.data_ptr(), nbytes)
+        context_lens.stride(0), out.data_ptr(), out.stride(), softmax_scale, workspace.data_ptr(), nbytes,
+        _status_word(device).data_ptr())
     _call(lib.fa_decode_paged8, p, device)
+    _lib.paged_binding().set_status(device.index, p.status)
     return out
 
 
@@ -225,6 +239,11 @@ def flash_attention_decode_paged_8bit(query, k_cache, v_cache, k_scales, v_scale
     Products and sums are fp32 over fp16 operands (keys and values are exact in fp16, probabilities are rounded to it).
     Non-causal, inference-only.
     """
+    if not torch.compiler.is_compiling():
+        out = _lib.paged_binding().decode(query, k_cache, v_cache, k_scales, v_scales, block_table, context_lens,
+                                          softmax_scale)
+        if out is not None:
+            return out
     validate_paged8_inputs(query, k_cache, v_cache, k_scales, v_scales, block_table, context_lens)
     validate_inference_only(query)
     validate_softmax_scale(softmax_scale)
@@ -259,6 +278,8 @@ class PagedKVCache8:
         self.v_cache = torch.zeros(shape, dtype=torch.int8, device=device).view(dtype)
         self.k_scales = torch.ones((layers, num_blocks, kv_heads), dtype=torch.float32, device=device)
         self.v_scales = torch.ones((layers, num_blocks, kv_heads), dtype=torch.float32, device=device)
+        self._layers = list(zip(self.k_cache.unbind(), self.v_cache.unbind(), self.k_scales.unbind(),
+                                self.v_scales.unbind()))
         self.block_table = torch.full((max_batch, max_blocks), -1, dtype=torch.int32, device=device)
         self.context_lens = torch.zeros(max_batch, dtype=torch.int32, device=device)
         self.free_blocks = torch.arange(num_blocks - 1, -1, -1, dtype=torch.int32, device=device)
@@ -272,11 +293,9 @@ class PagedKVCache8:
 
     def append(self, layer, key, value, slot_mapping):
         """`paged_kv_append` into one layer."""
-        paged_kv_append(key, value, self.k_cache[layer], self.v_cache[layer], self.k_scales[layer],
-                        self.v_scales[layer], slot_mapping)
+        paged_kv_append(key, value, *self._layers[layer], slot_mapping)
 
     def decode(self, layer, query, softmax_scale=None):
         """`flash_attention_decode_paged_8bit` of ``query`` ``(max_batch, q_heads, head_dim)`` against one layer."""
-        return flash_attention_decode_paged_8bit(query, self.k_cache[layer], self.v_cache[layer], self.k_scales[layer],
-                                                 self.v_scales[layer], self.block_table, self.context_lens,
+        return flash_attention_decode_paged_8bit(query, *self._layers[layer], self.block_table, self.context_lens,
                                                  softmax_scale)

@@ -297,6 +297,7 @@ typedef struct fa_paged8_params {
   void* out; int64_t o_strides[3];
   float softmax_scale;
   void* workspace; int64_t workspace_bytes;
+  int32_t* status;          /* device int32 or NULL, as in fa_decode_params */
 } fa_paged8_params;
 
 /* FP32 short-sequence attention: q, k, v, out (batch, heads, seqlen <= 32, 128), optional bias. */
