@@ -24,8 +24,8 @@
 namespace fa {
 namespace {
 
-constexpr int kWarps = 8;                       // compute warps; one more loads
-constexpr int kThreads = kWarps * 32 + 32;
+constexpr int kWarps = 8;                       // compute warps, two groups of four; the first warp of a third group loads
+constexpr int kThreads = kWarps * 32 + 128;
 constexpr int kStageBytes = 65536;              // K, then V
 constexpr int kStages = 3;
 constexpr int kMaxCtas = 256;
@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr int kRoundTiles = NT == 1 ? 4 : 2, kCols = kRoundTiles * 16;  // columns of a merge round
   constexpr int kHalfBytes = kStageBytes / 2 / T::kHalves;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ int64_t scan_s[kWarps + 1];
+  __shared__ int64_t scan_s[kWarps];
   __shared__ int64_t start_s[2];
   __shared__ __align__(8) uint64_t full_s[kStages], empty_s[kStages];
   __shared__ int plain_s[kStages];  // whether every token of the stage is there
@@ -199,11 +199,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int64_t x = __shfl_up_sync(0xffffffffu, sum, o);
       if (lane >= o) sum += x;
     }
-    if (lane == 31) scan_s[warp] = sum;
+    if (lane == 31 && warp < kWarps) scan_s[warp] = sum;
     __syncthreads();
     total = 0;
 #pragma unroll
-    for (int w = 0; w <= kWarps; ++w) {
+    for (int w = 0; w < kWarps; ++w) {
       if (w < warp) sum += scan_s[w];
       total += scan_s[w];
     }
@@ -248,8 +248,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   bool lost = false;
 
-  if (warp == kWarps) {
+  if (warp >= kWarps) {
     // =============================== producer warp ===============================
+    // (the CTA was launched with 168 registers a thread: 56 + 2 * 224 = 3 * 168)
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp > kWarps) return;
     const int box = 1 << a.box_shift, boxes = span >> a.box_shift, in_page = (1 << a.shift) - 1;
     const int entries = (span >> a.scale_shift) << a.head_shift;
     const uint32_t box_bytes = (uint32_t)(box << a.head_shift) * kRow;
@@ -327,6 +330,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     return;
   }
 
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
   // empty contexts have no unit: their rows are zeros
   for (int b = blockIdx.x; b < a.batch; b += gridDim.x)
     if (clamped_len(a, b) == 0)
@@ -737,9 +741,8 @@ constexpr int kMergeSplit = 4;
 template <int D, int NT>
 __global__ void __launch_bounds__(kMergeThreads) paged8_merge_kernel(const Args a) {
   constexpr int kVec = (D + 127) / 128;
-  __shared__ float weight_s[kMaxCtas];
   __shared__ float red_s[kMergeThreads / 32][D];
-  __shared__ float part_s[kMergeThreads / 32];
+  __shared__ float2 stat_s[kMergeThreads / 32];
   grid_dependency_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int4 cut = a.cuts[blockIdx.x + 1];
@@ -765,11 +768,9 @@ __global__ void __launch_bounds__(kMergeThreads) paged8_merge_kernel(const Args 
 #pragma unroll
       for (int p = 0; p < 8; ++p)
 #pragma unroll
-        for (int c = 0; c < kVec; ++c) {
-          x[p][c] = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (p < parts && lane * 4 + c * 128 < a.head_dim)
-            x[p][c] = *reinterpret_cast<const float4*>(a.part_o + part_row(p, row) * D + lane * 4 + c * 128);
-        }
+        for (int c = 0; c < kVec; ++c)
+          x[p][c] = *reinterpret_cast<const float4*>(a.part_o + part_row(min(p, parts - 1), row) * D +
+                                                     min(lane * 4 + c * 128, a.head_dim - 4));
       float2 st = make_float2(kNegInf, 0.f);
       if (lane < parts) st = *reinterpret_cast<const float2*>(a.part_stat + part_row(lane, row) * 2);
       float top = st.x;
@@ -800,55 +801,69 @@ __global__ void __launch_bounds__(kMergeThreads) paged8_merge_kernel(const Args 
     }
     return;
   }
+  constexpr int kMergeWarps = kMergeThreads / 32;
   for (int row = turn; row < rows; row += share) {
-    const float2 st = tid < parts ? *reinterpret_cast<const float2*>(a.part_stat + part_row(tid, row) * 2)
-                                  : make_float2(kNegInf, 0.f);
+    // warp w joins parts w, w + 8, ...; lane i holds the statistics of the i-th of them
+    const int64_t row_at = part_row(1, row) - 2 * slots;  // part p > 0 lies 2 * slots * p behind it, part 0 slots
+    auto part_at = [&](int p) { return row_at + (int64_t)(p == 0 ? 1 : 2 * p) * slots; };
+    const int mine = warp + kMergeWarps * lane, count = (parts - warp + kMergeWarps - 1) / kMergeWarps;
+    float2 st = make_float2(kNegInf, 0.f);
+    if (mine < parts) st = *reinterpret_cast<const float2*>(a.part_stat + part_at(mine) * 2);
     float top = st.x;
 #pragma unroll
     for (int i = 16; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
-    __syncthreads();
-    if (lane == 0) part_s[warp] = top;
-    __syncthreads();
-    for (int w = 0; w < kMergeThreads / 32; ++w) top = fmaxf(top, part_s[w]);
     const float w = fast_exp2(st.x - (top == kNegInf ? 0.f : top));
     float sum = w * st.y;
-    weight_s[tid] = w;
 #pragma unroll
     for (int i = 16; i > 0; i >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, i);
-    __syncthreads();
-    if (lane == 0) part_s[warp] = sum;
-    __syncthreads();
-    sum = 0.f;
-    for (int i = 0; i < kMergeThreads / 32; ++i) sum += part_s[i];
-    const float inverse = sum == 0.f ? 0.f : 1.f / sum;
+    float4 acc[kVec];
 #pragma unroll
-    for (int d = lane * 4; d < D; d += 128) {
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (d < a.head_dim) {
-#pragma unroll 8
-        for (int p = warp; p < parts; p += kMergeThreads / 32) {
-          const float f = weight_s[p];
-          const float4 x = *reinterpret_cast<const float4*>(a.part_o + part_row(p, row) * D + d);
-          acc.x += f * x.x;
-          acc.y += f * x.y;
-          acc.z += f * x.z;
-          acc.w += f * x.w;
+    for (int c = 0; c < kVec; ++c) acc[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+    // (clamped indexes instead of branches: the loads of a batch go out together)
+    for (int i0 = 0; i0 < count; i0 += 8) {
+      float4 x[8][kVec];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int c = 0; c < kVec; ++c)
+          x[i][c] = *reinterpret_cast<const float4*>(a.part_o + part_at(warp + kMergeWarps * min(i0 + i, count - 1)) * D +
+                                                     min(lane * 4 + c * 128, a.head_dim - 4));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float f = i0 + i < count ? __shfl_sync(0xffffffffu, w, (i0 + i) & 31) : 0.f;
+        if (i0 + i >= count) continue;
+#pragma unroll
+        for (int c = 0; c < kVec; ++c) {
+          acc[c].x += f * x[i][c].x;
+          acc[c].y += f * x[i][c].y;
+          acc[c].z += f * x[i][c].z;
+          acc[c].w += f * x[i][c].w;
         }
       }
-      *reinterpret_cast<float4*>(&red_s[warp][d]) = acc;
     }
+#pragma unroll
+    for (int c = 0; c < kVec; ++c)
+      if (lane * 4 + c * 128 < D) *reinterpret_cast<float4*>(&red_s[warp][lane * 4 + c * 128]) = acc[c];
+    if (lane == 0) stat_s[warp] = make_float2(top, sum);
     __syncthreads();
     if (tid * 4 < a.head_dim) {
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int i = 0; i < kMergeThreads / 32; ++i) {
-        const float4 x = *reinterpret_cast<const float4*>(&red_s[i][tid * 4]);
-        acc.x += x.x;
-        acc.y += x.y;
-        acc.z += x.z;
-        acc.w += x.w;
+      float all = kNegInf, norm = 0.f;
+      for (int i = 0; i < kMergeWarps; ++i) all = fmaxf(all, stat_s[i].x);
+      if (all == kNegInf) all = 0.f;
+      float4 total = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int i = 0; i < kMergeWarps; ++i) {
+        const float f = fast_exp2(stat_s[i].x - all);
+        const float4 y = *reinterpret_cast<const float4*>(&red_s[i][tid * 4]);
+        norm += f * stat_s[i].y;
+        total.x += f * y.x;
+        total.y += f * y.y;
+        total.z += f * y.z;
+        total.w += f * y.w;
       }
-      store4(row, tid * 4, make_float4(acc.x * inverse, acc.y * inverse, acc.z * inverse, acc.w * inverse));
+      const float inverse = norm == 0.f ? 0.f : 1.f / norm;
+      store4(row, tid * 4, make_float4(total.x * inverse, total.y * inverse, total.z * inverse, total.w * inverse));
     }
+    __syncthreads();
   }
 }
 
