@@ -31,6 +31,9 @@ struct CodeE4M3 {
         : "f"(a), "f"(b), "f"(c), "f"(d));
     return r;
   }
+  __device__ static __forceinline__ uint32_t pack4_times(float a, float b, float c, float d, float f) {
+    return pack4(a * f, b * f, c * f, d * f);
+  }
 };
 
 struct CodeInt8 {
@@ -50,6 +53,14 @@ struct CodeInt8 {
   __device__ static __forceinline__ int code(float v) { return max(-127, min(127, __float2int_rn(v))); }  // NaN: 0
   __device__ static __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
     return __byte_perm(__byte_perm(code(a), code(b), 0x0040), __byte_perm(code(c), code(d), 0x0040), 0x5410);
+  }
+  // Finite values times a power of two that takes them into the range: in 1.5 * 2^23 + x the sum's last bit is 1, so
+  // the addition rounds x to nearest even and leaves its two's complement in the low bits (four cvt would run at a
+  // quarter of the rate)
+  __device__ static __forceinline__ uint32_t pack4_times(float a, float b, float c, float d, float f) {
+    const uint32_t x = __float_as_uint(fmaf(a, f, 12582912.f)), y = __float_as_uint(fmaf(b, f, 12582912.f));
+    const uint32_t z = __float_as_uint(fmaf(c, f, 12582912.f)), w = __float_as_uint(fmaf(d, f, 12582912.f));
+    return __byte_perm(__byte_perm(x, y, 0x0040), __byte_perm(z, w, 0x0040), 0x5410);
   }
 };
 

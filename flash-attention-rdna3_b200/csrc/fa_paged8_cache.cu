@@ -15,11 +15,11 @@ int log2_of(int x) {
 // plan
 // ---------------------------------------------------------------------------------------------------
 // Everything follows from three running sums over the requests (new tokens, pages that come back, pages needed): every
-// CTA forms them for itself in shared memory, and tokens and pages then find their request by bisection. The CTAs are
-// one cluster, whose barrier separates the reads of the lengths from the writes, so that the lengths may be updated in
-// place.
+// CTA forms them for itself in shared memory, and tokens and pages then find their request there. Where the lengths are
+// updated in place the CTAs are one cluster, whose barrier separates the reads of the lengths from the writes.
 constexpr int kPlanThreads = 512;
 constexpr int kPlanMaxCluster = 8;
+constexpr int kPlanMaxCtas = 128;
 
 struct PlanArgs {
   int batch, max_blocks, num_blocks, shift, num_tokens;
@@ -58,46 +58,72 @@ __device__ __forceinline__ void block_scan2(int64_t& x, int64_t& y, int64_t* tx,
     part[warp][1] = y;
   }
   __syncthreads();
-  int64_t bx = 0, by = 0, sx = 0, sy = 0;
-  for (int w = 0; w < kPlanThreads / 32; ++w) {
-    if (w < warp) {
-      bx += part[w][0];
-      by += part[w][1];
-    }
-    sx += part[w][0];
-    sy += part[w][1];
+  // every warp adds the warps' totals up for itself (there are at most 32)
+  const int warps = blockDim.x >> 5;
+  int64_t vx = lane < warps ? part[lane][0] : 0, vy = lane < warps ? part[lane][1] : 0;
+  int64_t bx = lane < warp ? vx : 0, by = lane < warp ? vy : 0;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    if (o >= warps) continue;  // (uniform; warps is 1 for a small batch)
+    vx += __shfl_xor_sync(0xffffffffu, vx, o);
+    vy += __shfl_xor_sync(0xffffffffu, vy, o);
+    bx += __shfl_xor_sync(0xffffffffu, bx, o);
+    by += __shfl_xor_sync(0xffffffffu, by, o);
   }
-  x += bx;
-  y += by;
-  *tx = sx;
-  *ty = sy;
+  x += __shfl_sync(0xffffffffu, bx, 0);
+  y += __shfl_sync(0xffffffffu, by, 0);
+  *tx = __shfl_sync(0xffffffffu, vx, 0);
+  *ty = __shfl_sync(0xffffffffu, vy, 0);
 }
 
-// First index with ends[index] > value (n when there is none).
-__device__ __forceinline__ int first_above(const int* ends, int n, int value) {
-  int lo = 0, hi = n;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (ends[mid] > value) hi = mid;
-    else lo = mid + 1;
+// First index with ends[index] > value (n when there is none), for one value of the whole warp: 32 probes a round.
+__device__ __forceinline__ int warp_first_above(const int* ends, int n, int value) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, span = n;
+  while (span > 0) {
+    const int size = (span + 31) >> 5, probe = lo + (lane + 1) * size - 1;  // the last of 32 blocks' elements
+    const int below = __popc(__ballot_sync(0xffffffffu, probe < lo + span && ends[probe] <= value));
+    lo += below * size;
+    span = size == 1 ? 0 : min(size, span - below * size);
   }
   return lo;
 }
+// The same for a lane's own value, not below the warp's first one, whose index `known` is: within the next 32 entries by
+// shuffles, and by bisection in the shared array for lanes that lie behind them (empty entries can be many).
+__device__ __forceinline__ int lane_first_above(const int* ends, int n, int known, int value) {
+  const int lane = threadIdx.x & 31;
+  const int end = known + lane < n ? ends[known + lane] : INT32_MAX;
+  int index = 0;
+#pragma unroll
+  for (int w = 16; w > 0; w >>= 1)
+    if (__shfl_sync(0xffffffffu, end, index + w - 1) <= value) index += w;
+  if (__shfl_sync(0xffffffffu, end, 31) <= value) {
+    int lo = known + 32, hi = n;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (ends[mid] > value) hi = mid;
+      else lo = mid + 1;
+    }
+    return lo;
+  }
+  return known + index;
+}
 
+template <int kTogether>
 __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanArgs a) {
-  extern __shared__ int smem[];
+  extern __shared__ __align__(16) uint8_t smem[];
   __shared__ int64_t part[kPlanThreads / 32][2];
-  int* cu_end = smem;
+  int* cu_end = reinterpret_cast<int*>(smem);
   int* need_end = cu_end + a.batch;
   int* back_end = need_end + a.batch;
   int* len = back_end + a.batch;
   uint8_t* state = reinterpret_cast<uint8_t*>(len + a.batch);
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, threads = blockDim.x;
   const int64_t round_up = (1 << a.shift) - 1, capacity = (int64_t)a.max_blocks << a.shift;
   const int count = max(0, min(*a.count, a.num_blocks));
 
   int64_t fresh_sum = 0, back_sum = 0, need_sum = 0;
-  for (int c = 0; c < a.batch; c += kPlanThreads) {
+  for (int c = 0; c < a.batch; c += threads) {
     const int b = c + tid;
     const bool in = b < a.batch;
     const int64_t L = in ? a.lens[b * a.cl_stride] : 0, n = in ? a.fresh[b * a.nl_stride] : 0;
@@ -121,46 +147,73 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanArgs
   }
   const int available = saturated(count + back_sum);
   __syncthreads();
-  for (int b = tid; b < a.batch; b += kPlanThreads)
+  for (int b = tid; b < a.batch; b += threads)
     if (state[b] == kNeedsPages && need_end[b] > available) state[b] = kUnserved;
   __syncthreads();
   // every CTA has read the lengths and the count (and finished its own sums) before anyone writes
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 
-  uint32_t rank, ranks;
-  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
-  asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(ranks));
-  const int first = rank * kPlanThreads + tid, step = ranks * kPlanThreads;
+  const int first = blockIdx.x * threads + tid, step = gridDim.x * threads;
+  const int lane = tid & 31;
   // pages taken: the running need of the last request that is within what the stack holds
-  const int served_below = first_above(need_end, a.batch, available);
+  const int served_below = warp_first_above(need_end, a.batch, available);
   const int taken = served_below > 0 ? need_end[served_below - 1] : 0;
   const int left = available - taken;
 
-  // place `p` of the stack once the pages of ending requests lie on top of it
-  auto entry = [&](int p) -> int {
-    if (p < count) return a.stack[p];
-    const int k = p - count, b = first_above(back_end, a.batch, k);
-    return a.table[(int64_t)b * a.bt_stride + (k - (b > 0 ? back_end[b - 1] : 0))];
+  // Place `from` of the stack once the pages of ending requests lie on top of it. Nothing that is read here is written by
+  // this call: the stack below its old top, pages that requests held before, rows of ending requests.
+  auto entry = [&](int from) -> const int32_t* {
+    if (from < count) return a.stack + from;
+    const int k = from - count;
+    int lo = 0, hi = a.batch - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (back_end[mid] > k) hi = mid;
+      else lo = mid + 1;
+    }
+    return a.table + (int64_t)lo * a.bt_stride + (k - (lo > 0 ? back_end[lo - 1] : 0));
   };
 
-  for (int t = first; t < a.num_tokens; t += step) {
-    int64_t slot = -1;
-    const int b = first_above(cu_end, a.batch, t);
-    if (b < a.batch && (state[b] == kNeedsPages || state[b] == kNoPages)) {
+  // Slots, in groups of 32 tokens, kTogether of them at a time so that the loads of their page ids overlap. A group that
+  // lies in the request of the token before it needs no search; otherwise every lane looks for its own.
+  for (int64_t t0 = (int64_t)(first - lane) * kTogether; t0 < a.num_tokens; t0 += (int64_t)step * kTogether) {
+    const int32_t* from[kTogether];
+    int id[kTogether], offset[kTogether], known = warp_first_above(cu_end, a.batch, (int)t0);
+#pragma unroll
+    for (int k = 0; k < kTogether; ++k) {
+      const int64_t t_last = t0 + 32 * k + 31;
+      from[k] = nullptr;
+      offset[k] = 0;
+      if (t0 + 32 * k >= a.num_tokens) continue;
+      const int t = (int)min(t0 + 32 * k + lane, (int64_t)a.num_tokens - 1);
+      int b = known;
+      if (known < a.batch && cu_end[known] <= t_last) {
+        b = lane_first_above(cu_end, a.batch, known, t);
+        known = __shfl_sync(0xffffffffu, b, 31);
+      }
+      if (b >= a.batch || (state[b] != kNeedsPages && state[b] != kNoPages)) continue;
       const int pos = len[b] + (t - (b > 0 ? cu_end[b - 1] : 0));
       const int page = pos >> a.shift, have = (int)((len[b] + round_up) >> a.shift);
-      const int id = page < have ? a.table[(int64_t)b * a.bt_stride + page]
-                                 : entry(available - 1 - (b > 0 ? need_end[b - 1] : 0) - (page - have));
-      if (id >= 0 && id < a.num_blocks) slot = ((int64_t)id << a.shift) + (pos & (int)round_up);
+      offset[k] = pos & (int)round_up;
+      from[k] = page < have ? a.table + (int64_t)b * a.bt_stride + page
+                            : entry(available - 1 - (b > 0 ? need_end[b - 1] : 0) - (page - have));
     }
-    a.slots[t] = slot;
+#pragma unroll
+    for (int k = 0; k < kTogether; ++k) id[k] = from[k] != nullptr ? *from[k] : -1;
+#pragma unroll
+    for (int k = 0; k < kTogether; ++k)
+      if (t0 + 32 * k + lane < a.num_tokens)
+        a.slots[t0 + 32 * k + lane] = id[k] >= 0 && id[k] < a.num_blocks ? ((int64_t)id[k] << a.shift) + offset[k] : -1;
   }
-  for (int p = first; p < taken; p += step) {
-    const int b = first_above(need_end, a.batch, p);
+  // block-table entries of the new pages, and the places of the stack above its old top
+  for (int p0 = first - lane; p0 < taken; p0 += step) {
+    const int p = min(p0 + lane, taken - 1);
+    const int b = lane_first_above(need_end, a.batch, warp_first_above(need_end, a.batch, p0), p);
     const int have = (int)((len[b] + round_up) >> a.shift);
-    a.table[(int64_t)b * a.bt_stride + have + (p - (b > 0 ? need_end[b - 1] : 0))] = entry(available - 1 - p);
+    if (p0 + lane < taken)
+      a.table[(int64_t)b * a.bt_stride + have + (p - (b > 0 ? need_end[b - 1] : 0))] = *entry(available - 1 - p);
   }
-  for (int p = count + first; p < min(left, a.num_blocks); p += step) a.stack[p] = entry(p);
+  for (int p = count + first; p < min(left, a.num_blocks); p += step) a.stack[p] = *entry(p);
   for (int b = first; b < a.batch; b += step) {
     const int begin = b > 0 ? cu_end[b - 1] : 0;
     a.cu[b + 1] = cu_end[b];
@@ -200,17 +253,19 @@ template <typename T> struct Pair;
 template <> struct Pair<__half> { using type = __half2; };
 template <> struct Pair<__nv_bfloat16> { using type = __nv_bfloat162; };
 
-// Largest finite magnitude of eight 16-bit values, as fp32.
+// Largest finite magnitude of eight 16-bit values, as fp32; *special: some are not finite.
 template <typename T>
-__device__ __forceinline__ float finite_amax8(const uint4& v) {
+__device__ __forceinline__ float finite_amax8(const uint4& v, bool* special) {
   using P = typename Pair<T>::type;
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
   P m[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) m[i] = __habs2(*reinterpret_cast<const P*>(&w[i]));
-  const P r = __hmax2(__hmax2(m[0], m[1]), __hmax2(m[2], m[3]));  // a NaN loses against a number
-  float best = fmaxf(DType<T>::to_float(r.x), DType<T>::to_float(r.y));
-  if (!(best < INFINITY)) {
+  const P r = __hmax2_nan(__hmax2_nan(m[0], m[1]), __hmax2_nan(m[2], m[3]));
+  const float x = DType<T>::to_float(r.x), y = DType<T>::to_float(r.y);
+  float best = fmaxf(x, y);
+  if (!(x < INFINITY && y < INFINITY)) {
+    *special = true;
     best = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -231,7 +286,7 @@ __device__ __forceinline__ float scale_for(float amax) {
 }
 
 template <typename T, typename C8>
-__global__ void __launch_bounds__(kAppendThreads) paged8_append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(kAppendThreads, 4) paged8_append_kernel(const AppendArgs a) {
   __shared__ float part[2][kAppendWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int bs = 1 << a.shift;
@@ -288,6 +343,7 @@ __global__ void __launch_bounds__(kAppendThreads) paged8_append_kernel(const App
     const char* first_row = src + t_first * a.src_st[kv] * 2;
     uint4 held[kAppendLoads];
     float amax = 0.f;
+    bool special = false;
     for (int base = 0; base < n; base += chunk) {
 #pragma unroll
       for (int l = 0; l < kAppendLoads; ++l) {
@@ -297,7 +353,7 @@ __global__ void __launch_bounds__(kAppendThreads) paged8_append_kernel(const App
           held[l] = __ldg(reinterpret_cast<const uint4*>(first_row + j * a.src_st[kv] * 2));
       }
 #pragma unroll
-      for (int l = 0; l < kAppendLoads; ++l) amax = fmaxf(amax, finite_amax8<T>(held[l]));
+      for (int l = 0; l < kAppendLoads; ++l) amax = fmaxf(amax, finite_amax8<T>(held[l], &special));
     }
     amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));
     float* scale_at = a.scales[kv] + page * a.s_sb[kv] + head * a.s_sh[kv];
@@ -334,7 +390,7 @@ __global__ void __launch_bounds__(kAppendThreads) paged8_append_kernel(const App
 
     // ---- the new tokens. Dividing by a power of two is multiplying by its inverse; a scale that the caller made and
     // that is none is divided by.
-    const bool exact_inverse = (__float_as_uint(scale) & 0x7fffffu) == 0;
+    const bool simple = (__float_as_uint(scale) & 0x7fffffu) == 0 && !__any_sync(0xffffffffu, special);
     const float inverse = __fdiv_rn(1.f, scale);
     for (int base = 0; base < n; base += chunk) {
 #pragma unroll
@@ -344,19 +400,14 @@ __global__ void __launch_bounds__(kAppendThreads) paged8_append_kernel(const App
         uint4 v = held[l];
         if (n > chunk) v = __ldg(reinterpret_cast<const uint4*>(first_row + j * a.src_st[kv] * 2));
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-        float f[8];
+        uint32_t c[2];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float2 p = DType<T>::unpack2(w[k]);
-          f[2 * k] = p.x * inverse;
-          f[2 * k + 1] = p.y * inverse;
-          if (!exact_inverse) {
-            f[2 * k] = __fdiv_rn(p.x, scale);
-            f[2 * k + 1] = __fdiv_rn(p.y, scale);
-          }
+        for (int k = 0; k < 2; ++k) {
+          const float2 x = DType<T>::unpack2(w[2 * k]), y = DType<T>::unpack2(w[2 * k + 1]);
+          c[k] = simple ? C8::pack4_times(x.x, x.y, y.x, y.y, inverse)
+                        : C8::pack4(__fdiv_rn(x.x, scale), __fdiv_rn(x.y, scale), __fdiv_rn(y.x, scale), __fdiv_rn(y.y, scale));
         }
-        *reinterpret_cast<uint2*>(page_base + (offset + j) * a.c_st[kv] + col * 8) =
-            make_uint2(C8::pack4(f[0], f[1], f[2], f[3]), C8::pack4(f[4], f[5], f[6], f[7]));
+        *reinterpret_cast<uint2*>(page_base + (offset + j) * a.c_st[kv] + col * 8) = make_uint2(c[0], c[1]);
       }
     }
   }
@@ -392,29 +443,35 @@ int launch_paged_plan(const fa_paged_plan_params& p, cudaStream_t stream) {
   a.cu = p.cu_seqlens;
   a.lens_out = p.context_lens_out;
   a.count_out = p.free_count_out;
+  const bool inplace = a.lens_out == a.lens || a.count_out == a.count;
   const int smem = p.batch * 17;
   if (smem > 40 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    const cudaError_t e = inplace ? cudaFuncSetAttribute(paged_plan_kernel<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)
+                                  : cudaFuncSetAttribute(paged_plan_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) {
       cudaGetLastError();
       return set_error(FA_ERR_LAUNCH, "plan: cannot get %d bytes of shared memory: %s", smem, cudaGetErrorString(e));
     }
   }
+  // A thread for each request or token of a decode step; more CTAs for prompts, as many as there are groups of tokens for
+  // where the lengths are not updated in place, a cluster that takes four groups at a time where they are.
   const int64_t work = p.num_tokens > p.batch ? p.num_tokens : p.batch;
-  int cluster = 1;
-  while (cluster < kPlanMaxCluster && cluster * 2 * kPlanThreads <= work) cluster *= 2;
+  const int threads = work >= kPlanThreads ? kPlanThreads : (int)((work + 31) / 32 * 32);
+  int ctas = 1;
+  while (ctas < (inplace ? kPlanMaxCluster : kPlanMaxCtas) && ctas * kPlanThreads < work) ctas *= 2;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = cluster;
+  attr.val.clusterDim.x = ctas;
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(cluster);
-  cfg.blockDim = dim3(kPlanThreads);
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return check_launch("plan", cudaLaunchKernelEx(&cfg, paged_plan_kernel, a));
+  cfg.numAttrs = inplace ? 1 : 0;
+  return check_launch("plan", inplace ? cudaLaunchKernelEx(&cfg, paged_plan_kernel<4>, a)
+                                      : cudaLaunchKernelEx(&cfg, paged_plan_kernel<1>, a));
 }
 
 int launch_paged8_append(const fa_paged8_append_params& p, cudaStream_t stream) {
@@ -448,11 +505,13 @@ int launch_paged8_append(const fa_paged8_append_params& p, cudaStream_t stream) 
   const int rows = 32 / (p.head_dim / 8);
   a.warps = 1;
   while (a.warps < kAppendWarps && a.warps * kAppendLoads * rows < p.block_size) a.warps *= 2;
+  // (a few tokens are the single ones of a decode step: no more warps a task than there is room for at once)
+  while (a.warps > 1 && p.num_tokens <= 1024 && p.num_tokens * 2 * p.heads_kv * a.warps > 148 * 32) a.warps /= 2;
   const int64_t tasks = (2 * p.heads_kv + kAppendWarps / a.warps - 1) / (kAppendWarps / a.warps);
   if (tasks > 65535) return set_error(FA_ERR_UNSUPPORTED, "append: too many heads");
   // a CTA starts the runs of `range` tokens: one while the grid is small, up to a page's (at most 32) for prompts
   a.range = 1;
-  while (a.range < 32 && a.range < p.block_size && p.num_tokens * tasks / (2 * a.range) >= 1184) a.range *= 2;
+  while (a.range < 32 && a.range < p.block_size && p.num_tokens * tasks / (2 * a.range) >= 592) a.range *= 2;
   const int64_t grid = (p.num_tokens + a.range - 1) / a.range;
   if (grid > INT32_MAX) return set_error(FA_ERR_UNSUPPORTED, "append: too many tokens");
   const dim3 g((unsigned)grid, (unsigned)tasks);
