@@ -32,7 +32,19 @@ struct CodeE4M3 {
     return r;
   }
   __device__ static __forceinline__ uint32_t pack4_times(float a, float b, float c, float d, float f) {
-    return pack4(a * f, b * f, c * f, d * f);
+    const uint64_t ff = pack_f32x2(f, f), x = mul_f32x2(pack_f32x2(a, b), ff), y = mul_f32x2(pack_f32x2(c, d), ff);
+    unpack_f32x2(x, &a, &b);
+    unpack_f32x2(y, &c, &d);
+    return pack4(a, b, c, d);
+  }
+  // fp16 pairs times a power of two: exact, or below fp16's normal range, where every code is 0 (half of the smallest is 2^-10)
+  __device__ static __forceinline__ uint32_t pack4_half(__half2 lo, __half2 hi, __half2 f) {
+    const __half2 x = __hmul2(lo, f), y = __hmul2(hi, f);
+    uint32_t r;
+    asm("{.reg .b16 l, h; cvt.rn.satfinite.e4m3x2.f16x2 l, %1; cvt.rn.satfinite.e4m3x2.f16x2 h, %2; mov.b32 %0, {l, h};}"
+        : "=r"(r)
+        : "r"(*reinterpret_cast<const uint32_t*>(&x)), "r"(*reinterpret_cast<const uint32_t*>(&y)));
+    return r;
   }
 };
 
@@ -58,9 +70,18 @@ struct CodeInt8 {
   // the addition rounds x to nearest even and leaves its two's complement in the low bits (four cvt would run at a
   // quarter of the rate)
   __device__ static __forceinline__ uint32_t pack4_times(float a, float b, float c, float d, float f) {
-    const uint32_t x = __float_as_uint(fmaf(a, f, 12582912.f)), y = __float_as_uint(fmaf(b, f, 12582912.f));
-    const uint32_t z = __float_as_uint(fmaf(c, f, 12582912.f)), w = __float_as_uint(fmaf(d, f, 12582912.f));
-    return __byte_perm(__byte_perm(x, y, 0x0040), __byte_perm(z, w, 0x0040), 0x5410);
+    const uint64_t ff = pack_f32x2(f, f), magic = pack_f32x2(12582912.f, 12582912.f);
+    const uint64_t x = fma_f32x2(pack_f32x2(a, b), ff, magic), y = fma_f32x2(pack_f32x2(c, d), ff, magic);
+    unpack_f32x2(x, &a, &b);
+    unpack_f32x2(y, &c, &d);
+    return __byte_perm(__byte_perm(__float_as_uint(a), __float_as_uint(b), 0x0040),
+                       __byte_perm(__float_as_uint(c), __float_as_uint(d), 0x0040), 0x5410);
+  }
+  // The same in fp16, whose 1.5 * 2^10 + x has a last bit of 1 too: the product is exact inside the fused addition
+  __device__ static __forceinline__ uint32_t pack4_half(__half2 lo, __half2 hi, __half2 f) {
+    const __half2 magic = __half2half2(__ushort_as_half(0x6600));
+    const __half2 x = __hfma2(lo, f, magic), y = __hfma2(hi, f, magic);
+    return __byte_perm(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y), 0x6420);
   }
 };
 

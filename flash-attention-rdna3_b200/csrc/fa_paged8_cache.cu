@@ -2,6 +2,8 @@
 // and values into their pages (fa_paged8_append). include/fa_b200.h has the rules that both follow.
 #include "fa_paged8.cuh"
 
+#include <type_traits>
+
 namespace fa {
 namespace {
 
@@ -253,26 +255,23 @@ template <typename T> struct Pair;
 template <> struct Pair<__half> { using type = __half2; };
 template <> struct Pair<__nv_bfloat16> { using type = __nv_bfloat162; };
 
-// Largest finite magnitude of eight 16-bit values, as fp32; *special: some are not finite.
+// Eight 16-bit values as four pairs' magnitudes, into the running largest of each pair (NaN wins).
 template <typename T>
-__device__ __forceinline__ float finite_amax8(const uint4& v, bool* special) {
+__device__ __forceinline__ void amax8(const uint4& v, typename Pair<T>::type (&m)[4]) {
   using P = typename Pair<T>::type;
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-  P m[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) m[i] = __habs2(*reinterpret_cast<const P*>(&w[i]));
-  const P r = __hmax2_nan(__hmax2_nan(m[0], m[1]), __hmax2_nan(m[2], m[3]));
-  const float x = DType<T>::to_float(r.x), y = DType<T>::to_float(r.y);
-  float best = fmaxf(x, y);
-  if (!(x < INFINITY && y < INFINITY)) {
-    *special = true;
-    best = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = DType<T>::unpack2(w[i]);
-      if (fabsf(f.x) < INFINITY) best = fmaxf(best, fabsf(f.x));
-      if (fabsf(f.y) < INFINITY) best = fmaxf(best, fabsf(f.y));
-    }
+  for (int i = 0; i < 4; ++i) m[i] = __hmax2_nan(m[i], __habs2(*reinterpret_cast<const P*>(&w[i])));
+}
+// Largest finite magnitude of eight 16-bit values, some of which are not.
+template <typename T>
+__device__ __noinline__ float finite_amax8(const uint4 v) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  float best = 0.f;
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = DType<T>::unpack2(w[i]);
+    if (fabsf(f.x) < INFINITY) best = fmaxf(best, fabsf(f.x));
+    if (fabsf(f.y) < INFINITY) best = fmaxf(best, fabsf(f.y));
   }
   return best;
 }
@@ -285,8 +284,25 @@ __device__ __forceinline__ float scale_for(float amax) {
   return __uint_as_float((uint32_t)max(e, 1) << 23);
 }
 
+// Four 16-bit values -> four codes: times the inverse of a power of two (finite values; kHalf: fp16 values, and an inverse
+// that is an fp16 number, in fp16 arithmetic that rounds once), or divided by any scale.
+template <typename T, typename C8, bool kHalf>
+__device__ __forceinline__ uint32_t scaled4(uint32_t lo, uint32_t hi, float inverse) {
+  if constexpr (kHalf) {
+    const __half2 f = __float2half2_rn(inverse);
+    return C8::pack4_half(*reinterpret_cast<const __half2*>(&lo), *reinterpret_cast<const __half2*>(&hi), f);
+  }
+  const float2 x = DType<T>::unpack2(lo), y = DType<T>::unpack2(hi);
+  return C8::pack4_times(x.x, x.y, y.x, y.y, inverse);
+}
 template <typename T, typename C8>
-__global__ void __launch_bounds__(kAppendThreads, 4) paged8_append_kernel(const AppendArgs a) {
+__device__ __noinline__ uint32_t divided4(uint32_t lo, uint32_t hi, float scale) {
+  const float2 x = DType<T>::unpack2(lo), y = DType<T>::unpack2(hi);
+  return C8::pack4(__fdiv_rn(x.x, scale), __fdiv_rn(x.y, scale), __fdiv_rn(y.x, scale), __fdiv_rn(y.y, scale));
+}
+
+template <typename T, typename C8>
+__global__ void __launch_bounds__(kAppendThreads, 3) paged8_append_kernel(const AppendArgs a) {
   __shared__ float part[2][kAppendWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int bs = 1 << a.shift;
@@ -340,20 +356,34 @@ __global__ void __launch_bounds__(kAppendThreads, 4) paged8_append_kernel(const 
     n = min(n, bs - offset);
 
     // ---- largest magnitude of the run
-    const char* first_row = src + t_first * a.src_st[kv] * 2;
+    using P = typename Pair<T>::type;
+    const int64_t row_bytes = a.src_st[kv] * 2, load_step = rows * row_bytes;
+    const char* mine = src + t_first * row_bytes + (sub * kAppendLoads * rows + row) * row_bytes;
+    const int first_j = sub * kAppendLoads * rows + row, end_j = has_task && row < rows ? n : 0;  // a lane's rows, up to end_j
     uint4 held[kAppendLoads];
-    float amax = 0.f;
-    bool special = false;
+    const uint32_t none = 0u;
+    P m[4] = {*reinterpret_cast<const P*>(&none), *reinterpret_cast<const P*>(&none), *reinterpret_cast<const P*>(&none),
+              *reinterpret_cast<const P*>(&none)};
     for (int base = 0; base < n; base += chunk) {
+      const char* at = mine + base * row_bytes;
 #pragma unroll
-      for (int l = 0; l < kAppendLoads; ++l) {
-        const int j = base + (sub * kAppendLoads + l) * rows + row;
+      for (int l = 0; l < kAppendLoads; ++l, at += load_step) {
         held[l] = make_uint4(0u, 0u, 0u, 0u);
-        if (has_task && row < rows && j < n)
-          held[l] = __ldg(reinterpret_cast<const uint4*>(first_row + j * a.src_st[kv] * 2));
+        if (first_j + base + l * rows < end_j) held[l] = __ldg(reinterpret_cast<const uint4*>(at));
       }
 #pragma unroll
-      for (int l = 0; l < kAppendLoads; ++l) amax = fmaxf(amax, finite_amax8<T>(held[l], &special));
+      for (int l = 0; l < kAppendLoads; ++l) amax8<T>(held[l], m);
+    }
+    const P both = __hmax2_nan(__hmax2_nan(m[0], m[1]), __hmax2_nan(m[2], m[3]));
+    float amax = fmaxf(DType<T>::to_float(both.x), DType<T>::to_float(both.y));
+    const bool special = !(DType<T>::to_float(both.x) < INFINITY && DType<T>::to_float(both.y) < INFINITY);
+    if (special) {  // again, over the finite ones alone
+      amax = 0.f;
+      for (int j = first_j; j < end_j; j += rows) {
+        const int l = (j - first_j) / rows;
+        if (l % (kAppendLoads * a.warps) >= kAppendLoads) continue;  // other warps' rows
+        amax = fmaxf(amax, finite_amax8<T>(__ldg(reinterpret_cast<const uint4*>(mine + l * load_step))));
+      }
     }
     amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));
     float* scale_at = a.scales[kv] + page * a.s_sb[kv] + head * a.s_sh[kv];
@@ -392,22 +422,35 @@ __global__ void __launch_bounds__(kAppendThreads, 4) paged8_append_kernel(const 
     // that is none is divided by.
     const bool simple = (__float_as_uint(scale) & 0x7fffffu) == 0 && !__any_sync(0xffffffffu, special);
     const float inverse = __fdiv_rn(1.f, scale);
+    const int64_t store_step = rows * a.c_st[kv];
     for (int base = 0; base < n; base += chunk) {
+      const char* at = mine + base * row_bytes;
+      uint8_t* to = page_base + (int64_t)(offset + base + first_j) * a.c_st[kv] + col * 8;
+      if (simple) {
+        if (n > chunk) {
+          const char* again = at;
 #pragma unroll
-      for (int l = 0; l < kAppendLoads; ++l) {
-        const int j = base + (sub * kAppendLoads + l) * rows + row;
-        if (row >= rows || j >= n) continue;
-        uint4 v = held[l];
-        if (n > chunk) v = __ldg(reinterpret_cast<const uint4*>(first_row + j * a.src_st[kv] * 2));
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-        uint32_t c[2];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const float2 x = DType<T>::unpack2(w[2 * k]), y = DType<T>::unpack2(w[2 * k + 1]);
-          c[k] = simple ? C8::pack4_times(x.x, x.y, y.x, y.y, inverse)
-                        : C8::pack4(__fdiv_rn(x.x, scale), __fdiv_rn(x.y, scale), __fdiv_rn(y.x, scale), __fdiv_rn(y.y, scale));
+          for (int l = 0; l < kAppendLoads; ++l, again += load_step)
+            if (first_j + base + l * rows < end_j) held[l] = __ldg(reinterpret_cast<const uint4*>(again));
         }
-        *reinterpret_cast<uint2*>(page_base + (offset + j) * a.c_st[kv] + col * 8) = make_uint2(c[0], c[1]);
+        auto store = [&](auto half) {
+#pragma unroll
+          for (int l = 0; l < kAppendLoads; ++l, to += store_step)
+            if (first_j + base + l * rows < end_j)
+              *reinterpret_cast<uint2*>(to) = make_uint2(scaled4<T, C8, decltype(half)::value>(held[l].x, held[l].y, inverse),
+                                                         scaled4<T, C8, decltype(half)::value>(held[l].z, held[l].w, inverse));
+        };
+        if (std::is_same<T, __half>::value && inverse <= 32768.f && inverse >= 6.103515625e-05f)
+          store(std::integral_constant<bool, std::is_same<T, __half>::value>());
+        else
+          store(std::false_type());
+      } else {
+#pragma unroll 1
+        for (int l = 0; l < kAppendLoads; ++l, to += store_step)
+          if (first_j + base + l * rows < end_j) {
+            const uint4 v = __ldg(reinterpret_cast<const uint4*>(at + l * load_step));
+            *reinterpret_cast<uint2*>(to) = make_uint2(divided4<T, C8>(v.x, v.y, scale), divided4<T, C8>(v.z, v.w, scale));
+          }
       }
     }
   }
@@ -506,7 +549,7 @@ int launch_paged8_append(const fa_paged8_append_params& p, cudaStream_t stream) 
   a.warps = 1;
   while (a.warps < kAppendWarps && a.warps * kAppendLoads * rows < p.block_size) a.warps *= 2;
   // (a few tokens are the single ones of a decode step: no more warps a task than there is room for at once)
-  while (a.warps > 1 && p.num_tokens <= 1024 && p.num_tokens * 2 * p.heads_kv * a.warps > 148 * 32) a.warps /= 2;
+  while (a.warps > 1 && p.num_tokens <= 1024 && p.num_tokens * 2 * p.heads_kv * a.warps > 148 * 3 * kAppendWarps) a.warps /= 2;
   const int64_t tasks = (2 * p.heads_kv + kAppendWarps / a.warps - 1) / (kAppendWarps / a.warps);
   if (tasks > 65535) return set_error(FA_ERR_UNSUPPORTED, "append: too many heads");
   // a CTA starts the runs of `range` tokens: one while the grid is small, up to a page's (at most 32) for prompts
