@@ -1,6 +1,7 @@
 // The two operators that fill a paged 8-bit cache: page and slot planning (fa_paged_plan) and the rounding of new keys
 // and values into their pages (fa_paged8_append). include/fa_b200.h has the rules that both follow.
 #include "fa_paged8.cuh"
+#include "fa_sm100.cuh"
 
 #include <type_traits>
 
@@ -121,6 +122,8 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanArgs
   int* len = back_end + a.batch;
   uint8_t* state = reinterpret_cast<uint8_t*>(len + a.batch);
   const int tid = threadIdx.x, threads = blockDim.x;
+  grid_launch_dependents();
+  grid_dependency_wait();  // (launched while the kernel before it ends)
   const int64_t round_up = (1 << a.shift) - 1, capacity = (int64_t)a.max_blocks << a.shift;
   const int count = max(0, min(*a.count, a.num_blocks));
 
@@ -304,6 +307,8 @@ __device__ __noinline__ uint32_t divided4(uint32_t lo, uint32_t hi, float scale)
 template <typename T, typename C8>
 __global__ void __launch_bounds__(kAppendThreads, 3) paged8_append_kernel(const AppendArgs a) {
   __shared__ float part[2][kAppendWarps];
+  grid_launch_dependents();
+  grid_dependency_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int bs = 1 << a.shift;
   const int64_t t0 = (int64_t)blockIdx.x * a.range;
@@ -502,17 +507,19 @@ int launch_paged_plan(const fa_paged_plan_params& p, cudaStream_t stream) {
   const int threads = work >= kPlanThreads ? kPlanThreads : (int)((work + 31) / 32 * 32);
   int ctas = 1;
   while (ctas < (inplace ? kPlanMaxCluster : kPlanMaxCtas) && ctas * kPlanThreads < work) ctas *= 2;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = ctas;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchAttribute attrs[2];
+  attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attrs[0].val.programmaticStreamSerializationAllowed = 1;
+  attrs[1].id = cudaLaunchAttributeClusterDimension;
+  attrs[1].val.clusterDim.x = ctas;
+  attrs[1].val.clusterDim.y = attrs[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cfg.attrs = &attr;
-  cfg.numAttrs = inplace ? 1 : 0;
+  cfg.attrs = attrs;
+  cfg.numAttrs = inplace ? 2 : 1;
   return check_launch("plan", inplace ? cudaLaunchKernelEx(&cfg, paged_plan_kernel<4>, a)
                                       : cudaLaunchKernelEx(&cfg, paged_plan_kernel<1>, a));
 }
@@ -557,16 +564,25 @@ int launch_paged8_append(const fa_paged8_append_params& p, cudaStream_t stream) 
   while (a.range < 32 && a.range < p.block_size && p.num_tokens * tasks / (2 * a.range) >= 592) a.range *= 2;
   const int64_t grid = (p.num_tokens + a.range - 1) / a.range;
   if (grid > INT32_MAX) return set_error(FA_ERR_UNSUPPORTED, "append: too many tokens");
-  const dim3 g((unsigned)grid, (unsigned)tasks);
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid, (unsigned)tasks);
+  cfg.blockDim = dim3(kAppendThreads);
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
   const bool e4m3 = p.cache_dtype == FA_CACHE_E4M3;
+  cudaError_t e;
   if (p.dtype == FA_F16) {
-    if (e4m3) paged8_append_kernel<__half, CodeE4M3><<<g, kAppendThreads, 0, stream>>>(a);
-    else paged8_append_kernel<__half, CodeInt8><<<g, kAppendThreads, 0, stream>>>(a);
+    e = e4m3 ? cudaLaunchKernelEx(&cfg, paged8_append_kernel<__half, CodeE4M3>, a)
+             : cudaLaunchKernelEx(&cfg, paged8_append_kernel<__half, CodeInt8>, a);
   } else {
-    if (e4m3) paged8_append_kernel<__nv_bfloat16, CodeE4M3><<<g, kAppendThreads, 0, stream>>>(a);
-    else paged8_append_kernel<__nv_bfloat16, CodeInt8><<<g, kAppendThreads, 0, stream>>>(a);
+    e = e4m3 ? cudaLaunchKernelEx(&cfg, paged8_append_kernel<__nv_bfloat16, CodeE4M3>, a)
+             : cudaLaunchKernelEx(&cfg, paged8_append_kernel<__nv_bfloat16, CodeInt8>, a);
   }
-  return check_launch("append", cudaSuccess);
+  return check_launch("append", e);
 }
 
 }  // namespace fa

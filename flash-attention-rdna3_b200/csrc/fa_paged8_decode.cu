@@ -184,7 +184,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&empty_s[i], kWarps);
     }
     mbar_fence_init();
+    tma_prefetch_desc(&k_map);
+    tma_prefetch_desc(&v_map);
   }
+  grid_dependency_wait();  // nothing above touches global memory: it runs while the kernel before this one ends
 
   // ---- this CTA's stretch of units
   int64_t total, u_begin, u_end;
@@ -263,13 +266,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     auto fetch = [&]() -> int { return lane < boxes ? page_at(at.step * span + lane * box) : -1; };
     int page = -1;
-    if (units > 0) {
-      page = fetch();
-      if (lane == 0) {
-        tma_prefetch_desc(&k_map);
-        tma_prefetch_desc(&v_map);
-      }
-    }
+    if (units > 0) page = fetch();
     int stage = 0, issued = 0;
     uint32_t parity = 1;
     for (; issued < units; ++issued) {
@@ -743,6 +740,7 @@ __global__ void __launch_bounds__(kMergeThreads) paged8_merge_kernel(const Args 
   constexpr int kVec = (D + 127) / 128;
   __shared__ float red_s[kMergeThreads / 32][D];
   __shared__ float2 stat_s[kMergeThreads / 32];
+  grid_launch_dependents();
   grid_dependency_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int4 cut = a.cuts[blockIdx.x + 1];
@@ -764,6 +762,8 @@ __global__ void __launch_bounds__(kMergeThreads) paged8_merge_kernel(const Args 
 
   if (parts <= 8) {
     for (int row = turn + share * warp; row < rows; row += share * (kMergeThreads / 32)) {
+      float2 st = make_float2(kNegInf, 0.f);
+      if (lane < parts) st = *reinterpret_cast<const float2*>(a.part_stat + part_row(lane, row) * 2);
       float4 x[8][kVec];
 #pragma unroll
       for (int p = 0; p < 8; ++p)
@@ -771,8 +771,6 @@ __global__ void __launch_bounds__(kMergeThreads) paged8_merge_kernel(const Args 
         for (int c = 0; c < kVec; ++c)
           x[p][c] = *reinterpret_cast<const float4*>(a.part_o + part_row(min(p, parts - 1), row) * D +
                                                      min(lane * 4 + c * 128, a.head_dim - 4));
-      float2 st = make_float2(kNegInf, 0.f);
-      if (lane < parts) st = *reinterpret_cast<const float2*>(a.part_stat + part_row(lane, row) * 2);
       float top = st.x;
 #pragma unroll
       for (int i = 4; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
@@ -807,8 +805,18 @@ __global__ void __launch_bounds__(kMergeThreads) paged8_merge_kernel(const Args 
     const int64_t row_at = part_row(1, row) - 2 * slots;  // part p > 0 lies 2 * slots * p behind it, part 0 slots
     auto part_at = [&](int p) { return row_at + (int64_t)(p == 0 ? 1 : 2 * p) * slots; };
     const int mine = warp + kMergeWarps * lane, count = (parts - warp + kMergeWarps - 1) / kMergeWarps;
+    float4 x[8][kVec];
+    auto load = [&](int i0) {  // (clamped indexes instead of branches: the loads of a batch go out together)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int c = 0; c < kVec; ++c)
+          x[i][c] = *reinterpret_cast<const float4*>(a.part_o + part_at(warp + kMergeWarps * min(i0 + i, count - 1)) * D +
+                                                     min(lane * 4 + c * 128, a.head_dim - 4));
+    };
     float2 st = make_float2(kNegInf, 0.f);
     if (mine < parts) st = *reinterpret_cast<const float2*>(a.part_stat + part_at(mine) * 2);
+    load(0);
     float top = st.x;
 #pragma unroll
     for (int i = 16; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
@@ -819,15 +827,8 @@ __global__ void __launch_bounds__(kMergeThreads) paged8_merge_kernel(const Args 
     float4 acc[kVec];
 #pragma unroll
     for (int c = 0; c < kVec; ++c) acc[c] = make_float4(0.f, 0.f, 0.f, 0.f);
-    // (clamped indexes instead of branches: the loads of a batch go out together)
     for (int i0 = 0; i0 < count; i0 += 8) {
-      float4 x[8][kVec];
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-#pragma unroll
-        for (int c = 0; c < kVec; ++c)
-          x[i][c] = *reinterpret_cast<const float4*>(a.part_o + part_at(warp + kMergeWarps * min(i0 + i, count - 1)) * D +
-                                                     min(lane * 4 + c * 128, a.head_dim - 4));
+      if (i0 > 0) load(i0);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float f = i0 + i < count ? __shfl_sync(0xffffffffu, w, (i0 + i) & 31) : 0.f;
@@ -917,20 +918,21 @@ int launch(const CUtensorMap& k, const CUtensorMap& v, const Args& a, int ctas, 
   constexpr int smem = Smem<D, NT>::kBytes;
   static_assert(smem <= 227 * 1024 - 512, "shared memory of an SM");
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e == cudaSuccess) {
-    kernel<<<ctas, kThreads, smem, stream>>>(k, v, a);
-    e = cudaGetLastError();
-  }
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, kernel, k, v, a);
   if (e == cudaSuccess && ctas > 1) {
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas - 1, kMergeSplit);
     cfg.blockDim = dim3(kMergeThreads);
-    cfg.stream = stream;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
+    cfg.dynamicSmemBytes = 0;
     e = cudaLaunchKernelEx(&cfg, paged8_merge_kernel<D, NT>, a);
   }
   if (e == cudaSuccess) return 0;

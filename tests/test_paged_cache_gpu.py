@@ -590,3 +590,52 @@ def test_inference_only():
         fa_b200.flash_attention_decode_paged_8bit(*d)
     with torch.no_grad():
         fa_b200.flash_attention_decode_paged_8bit(*d)
+
+
+def test_captured_behind_copies_and_joined_streams():
+    """The kernels start early behind whatever precedes them: a copy, a fill, a kernel of another stream, in a graph and
+    outside, never before it has written what they read."""
+    args = decode_case(21, [700, 90, 1], 8, 2, 64, 16, torch.float16, E4M3)
+    sources = [[t.clone() for t in decode_case(s, [700, 90, 1], 8, 2, 64, 16, torch.float16, E4M3)] for s in (22, 23)]
+    plan = random_plan(31, 40, 16, 20, 60, 90)
+    side = torch.cuda.Stream()
+
+    def step(src):
+        for t, u in zip(args[:5], src):                       # copies, then fills, right in front
+            t.copy_(u)
+        out = fa_b200.flash_attention_decode_paged_8bit(*args)
+        args[0].zero_()
+        zero = fa_b200.flash_attention_decode_paged_8bit(*args)
+        here = torch.cuda.current_stream()
+        side.wait_stream(here)
+        with torch.cuda.stream(side):
+            args[0].copy_(src[0])
+            other = fa_b200.flash_attention_decode_paged_8bit(*args)
+            slots = fa_b200.paged_kv_plan(*plan, 16)[0]
+        here.wait_stream(side)
+        last = fa_b200.flash_attention_decode_paged_8bit(*args)
+        x = args[1][0].float().half()
+        fa_b200.paged_kv_append(x, -x, args[1], args[2], args[3], args[4], torch.arange(16, 32, device="cuda"))
+        after = fa_b200.flash_attention_decode_paged_8bit(*args)
+        return out, zero, other, last, after, slots
+
+    want = []
+    for src in sources:
+        torch.cuda.synchronize()
+        want.append([t.clone() for t in step(src)])
+        torch.cuda.synchronize()
+        full = [*src[:5], args[5], args[6]]
+        assert torch.equal(want[-1][0], fa_b200.flash_attention_decode_paged_8bit(*full))
+        assert torch.equal(want[-1][2], want[-1][0]) and torch.equal(want[-1][3], want[-1][0])
+    live = [t.clone() for t in sources[0]]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(live)
+    for _ in range(5):
+        for src, ref in zip(sources, want):
+            for t, u in zip(live, src):
+                t.copy_(u)
+            graph.replay()
+            torch.cuda.synchronize()
+            for a, b in zip(got, ref):
+                assert torch.equal(a, b)
