@@ -104,7 +104,7 @@ def _build_binding(force, verbose, header_time):
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            f"-I{sysconfig.get_paths()['include']}",
            *(f"-isystem{d}" for d in cpp_extension.include_paths("cuda")), f"-L{lib}",
-           "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-Wl,--as-needed"]
+           "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-Wl,--as-needed"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if verbose or r.returncode != 0:
         sys.stderr.write(f"--- fa_paged8_bind.cpp\n{r.stdout}{r.stderr}\n")

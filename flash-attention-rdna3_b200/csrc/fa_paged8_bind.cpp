@@ -6,6 +6,7 @@
 // anything. None means "not this way": tensors that break a contract (Python then finds and names it), that need a copy
 // first, that are traced or not ordinary tensors. Nothing here words an error but the library's own.
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/GradMode.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -114,7 +115,7 @@ void launch(F fn, const P& p, int device) {
 }
 
 at::Tensor empty(at::IntArrayRef sizes, at::ScalarType type, int device) {
-  return at::empty(sizes, at::TensorOptions().dtype(type).device(c10::Device(c10::kCUDA, device)));
+  return at::detail::empty_cuda(sizes, type, c10::Device(c10::kCUDA, device), std::nullopt);
 }
 
 // A plain Python int (a bool is none), or -1.

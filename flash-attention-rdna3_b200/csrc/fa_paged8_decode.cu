@@ -17,6 +17,8 @@
 // workspace, and paged8_merge_kernel joins the parts in the order of the stretches.
 #include <cuda.h>
 
+#include <atomic>
+
 #include "fa_paged8.cuh"
 #include "fa_sm100.cuh"
 #include "fa_tma_host.h"
@@ -886,14 +888,26 @@ Shape shape_of(const fa_paged8_params& p) {
   return s;
 }
 
+// What the host asks the driver once per device (the answers cannot change): a call costs about half a microsecond.
+constexpr int kMaxDevices = 64;
+int current_device() {
+  int dev = 0;
+  if (cudaGetDevice(&dev) == cudaSuccess) return dev;
+  cudaGetLastError();
+  return -1;
+}
 int cta_count() {
-  int dev = 0, sms = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0) {
+  static std::atomic<int> known[kMaxDevices];
+  const int dev = current_device();
+  if (dev >= 0 && dev < kMaxDevices && known[dev].load(std::memory_order_relaxed) > 0) return known[dev].load(std::memory_order_relaxed);
+  int sms = 0;
+  if (dev < 0 || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0) {
     cudaGetLastError();
     return set_error(FA_ERR_DEVICE, "cannot query the SM count of the current device");
   }
-  return sms < kMaxCtas ? sms : kMaxCtas;
+  sms = sms < kMaxCtas ? sms : kMaxCtas;
+  if (dev < kMaxDevices) known[dev].store(sms, std::memory_order_relaxed);
+  return sms;
 }
 
 // (dim, token of the page, head, page) with a box of one row's bytes x a box's tokens x a CTA's heads
@@ -917,7 +931,13 @@ int launch(const CUtensorMap& k, const CUtensorMap& v, const Args& a, int ctas, 
   auto kernel = paged8_kernel<C8, D, NT>;
   constexpr int smem = Smem<D, NT>::kBytes;
   static_assert(smem <= 227 * 1024 - 512, "shared memory of an SM");
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static std::atomic<bool> prepared[kMaxDevices];
+  const int dev = current_device();
+  cudaError_t e = cudaSuccess;
+  if (dev < 0 || dev >= kMaxDevices || !prepared[dev].load(std::memory_order_relaxed)) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess && dev >= 0 && dev < kMaxDevices) prepared[dev].store(true, std::memory_order_relaxed);
+  }
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
