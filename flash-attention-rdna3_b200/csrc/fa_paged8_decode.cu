@@ -696,7 +696,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               put4(nt * 8 + 2 * t4 + e, (i / 8) * 128 + kPerLane * g + 2 * (i % 8),
                    make_float4(o[nt][i][e] * weight[nt][e], o[nt][i][2 + e] * weight[nt][e],
                                o[nt][i + 1][e] * weight[nt][e], o[nt][i + 1][2 + e] * weight[nt][e]));
-      } else {
+      } else {  // sums of the head's warps, kRoundTiles tiles of dimensions at a time (rolled loops: this code runs once an item)
         float* mine = merge + warp * 512;
 #pragma unroll
         for (int round = 0; round < kNm / kRoundTiles; ++round) {
@@ -711,10 +711,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                     make_float2(x[e] * weight[nt][e], x[2 + e] * weight[nt][e]);
               }
           head_barrier(1 + wh, warps_head * 32);
+#pragma unroll 1
           for (int x = wt * 32 + lane; x < 128; x += warps_head * 32) {
             const int row = x * 4 / kCols, col = x * 4 % kCols;
             const float* from = merge + (warp - wt) * 512 + x * 4;
             float4 acc = *reinterpret_cast<const float4*>(from);
+#pragma unroll 1
             for (int w = 1; w < warps_head; ++w) {
               const float4 y = *reinterpret_cast<const float4*>(from + w * 512);
               acc.x += y.x;
