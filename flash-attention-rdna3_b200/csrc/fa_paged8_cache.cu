@@ -239,6 +239,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanArgs
 constexpr int kAppendThreads = 256;
 constexpr int kAppendWarps = kAppendThreads / 32;
 constexpr int kAppendLoads = 8;
+constexpr int kAppendWindow = 512;  // slots that a CTA looks at: up to 256 that may start a run, and those behind them
 
 struct AppendArgs {
   int heads, head_dim, shift, range, warps;  // range: tokens whose runs a CTA starts; warps: warps a task
@@ -304,13 +305,17 @@ __device__ __noinline__ uint32_t divided4(uint32_t lo, uint32_t hi, float scale)
   return C8::pack4(__fdiv_rn(x.x, scale), __fdiv_rn(x.y, scale), __fdiv_rn(y.x, scale), __fdiv_rn(y.y, scale));
 }
 
-template <typename T, typename C8>
+template <typename T, typename C8, bool kWide>
 __global__ void __launch_bounds__(kAppendThreads, 3) paged8_append_kernel(const AppendArgs a) {
   __shared__ float part[2][kAppendWarps];
   grid_launch_dependents();
   grid_dependency_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int bs = 1 << a.shift;
+  __shared__ int64_t slot_s[kWide ? kAppendWindow + 1 : 1];  // from the token in front of the range on; -1: none
+  __shared__ int16_t start_s[kAppendThreads];
+  __shared__ int count_s[kAppendWarps];
+  [[maybe_unused]] const int tid = threadIdx.x;
   const int64_t t0 = (int64_t)blockIdx.x * a.range;
   const int task = blockIdx.y * (kAppendWarps / a.warps) + warp / a.warps, sub = warp % a.warps;
   const bool has_task = task < 2 * a.heads;
@@ -322,40 +327,87 @@ __global__ void __launch_bounds__(kAppendThreads, 3) paged8_append_kernel(const 
   uint8_t* cache = a.cache[kv] + head * a.c_sh[kv];
   const int lanes8 = a.head_dim / 16, rows8 = 32 / lanes8;
 
-  // Runs that start in [t0, t0 + range): neighbours with slots in the same page. Every warp finds the same ones.
+  // Runs that start in [t0, t0 + range): neighbours with slots in the same page.
   auto slot_at = [&](int64_t t) -> int64_t {
     const int64_t s = t >= 0 && t < a.num_tokens ? a.slots[t * a.slot_stride] : -1;
     return s >= 0 && s < a.num_slots ? s : -1;
   };
-  int64_t s = slot_at(t0 + lane);
-  int64_t before = __shfl_up_sync(0xffffffffu, s, 1);
-  if (lane == 0) before = slot_at(t0 - 1);
-  const bool same = s >= 0 && before >= 0 && (s >> a.shift) == (before >> a.shift);
-  bool disorder = same && s != before + 1;
-  uint32_t starts = __ballot_sync(0xffffffffu, s >= 0 && !same && lane < a.range);
-  const uint32_t breaks = __ballot_sync(0xffffffffu, !same);
+  // A warp a task (kWide false): every warp finds the runs by itself, and none waits for another. Several warps a task, pages
+  // of more tokens: the CTA finds them together, over ranges of up to 256 tokens.
+  int64_t s = -1;
+  uint32_t starts = 0u, breaks = 0u;
+  bool disorder = false;
+  int runs = 0;
+  const int window = min(a.range + bs, kAppendWindow);
+  if constexpr (!kWide) {
+    s = slot_at(t0 + lane);
+    int64_t before = __shfl_up_sync(0xffffffffu, s, 1);
+    if (lane == 0) before = slot_at(t0 - 1);
+    const bool same = s >= 0 && before >= 0 && (s >> a.shift) == (before >> a.shift);
+    disorder = same && s != before + 1;
+    starts = __ballot_sync(0xffffffffu, s >= 0 && !same && lane < a.range);
+    breaks = __ballot_sync(0xffffffffu, !same);
+    runs = __popc(starts);
+  } else {
+    for (int i = tid; i <= window; i += kAppendThreads) slot_s[i] = slot_at(t0 - 1 + i);
+    __syncthreads();
+    {
+      const int64_t mine = tid < a.range ? slot_s[tid + 1] : -1, before = slot_s[min(tid, window)];
+      const bool same = mine >= 0 && before >= 0 && (mine >> a.shift) == (before >> a.shift);
+      disorder = same && mine != before + 1;
+      const bool start = mine >= 0 && !same;
+      const uint32_t mask = __ballot_sync(0xffffffffu, start);
+      if (lane == 0) count_s[warp] = __popc(mask);
+      __syncthreads();
+      int at = __popc(mask & ((1u << lane) - 1));
+      for (int w = 0; w < warp; ++w) at += count_s[w];
+      if (start) start_s[at] = (int16_t)tid;
+    }
+    __syncthreads();
+    for (int w = 0; w < kAppendWarps; ++w) runs += count_s[w];
 
-  int round = 0;
-  while (starts) {
-    const int i = __ffs(starts) - 1;
-    starts &= starts - 1;
-    const int64_t slot = __shfl_sync(0xffffffffu, s, i);
+  }
+  if (disorder && a.status != nullptr) *a.status = FA_STATUS_SLOT_ORDER;
+
+  for (int run = 0; run < runs; ++run) {
+    int i;
+    int64_t slot;
+    if constexpr (!kWide) {
+      i = __ffs(starts) - 1;
+      starts &= starts - 1;
+      slot = __shfl_sync(0xffffffffu, s, i);
+    } else {
+      i = start_s[run];
+      slot = slot_s[i + 1];
+    }
     const int64_t page = slot >> a.shift, t_first = t0 + i;
     const int offset = (int)(slot & (bs - 1));
-    const uint32_t later = i == 31 ? 0u : breaks & (0xffffffffu << (i + 1));
     int n;
-    if (later) {
-      n = __ffs(later) - 1 - i;
+    if constexpr (!kWide) {
+      const uint32_t later = i == 31 ? 0u : breaks & (0xffffffffu << (i + 1));
+      if (later) {
+        n = __ffs(later) - 1 - i;
+      } else {
+        n = 32 - i;
+        for (int64_t t = t0 + 32; n < bs; t += 32) {  // the run leaves the window
+          const int64_t x = slot_at(t + lane);
+          const bool cont = x >= 0 && (x >> a.shift) == page;
+          const uint32_t stop = __ballot_sync(0xffffffffu, !cont);
+          const int more = stop ? __ffs(stop) - 1 : 32;
+          n += more;
+          if (stop) break;
+        }
+      }
     } else {
-      n = 32 - i;
-      for (int64_t t = t0 + 32; n < bs; t += 32) {  // the run leaves the window
-        const int64_t x = slot_at(t + lane), y = slot_at(t + lane - 1);
-        const bool cont = x >= 0 && (x >> a.shift) == page;
-        const uint32_t stop = __ballot_sync(0xffffffffu, !cont);
-        const int more = stop ? __ffs(stop) - 1 : 32;
-        if (lane < more && x != y + 1) disorder = true;
-        n += more;
-        if (stop) break;
+      n = 1;
+      for (; n < bs - offset; n += 32) {
+        const int x = i + n + lane;
+        const int64_t next = x < window ? slot_s[x + 1] : slot_at(t0 + x);
+        const uint32_t stop = __ballot_sync(0xffffffffu, next < 0 || (next >> a.shift) != page);
+        if (stop) {
+          n += __ffs(stop) - 1;
+          break;
+        }
       }
     }
     n = min(n, bs - offset);
@@ -393,11 +445,10 @@ __global__ void __launch_bounds__(kAppendThreads, 3) paged8_append_kernel(const 
     amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));
     float* scale_at = a.scales[kv] + page * a.s_sb[kv] + head * a.s_sh[kv];
     const float old = offset > 0 ? *scale_at : 0.f;
-    if (a.warps > 1) {
-      if (lane == 0) part[round & 1][warp] = amax;
+    if constexpr (kWide) {
+      if (lane == 0) part[run & 1][warp] = amax;
       __syncthreads();  // also: every warp of the task has read the old scale
-      for (int w = 0; w < a.warps; ++w) amax = fmaxf(amax, part[round & 1][warp - sub + w]);
-      ++round;
+      for (int w = 0; w < a.warps; ++w) amax = fmaxf(amax, part[run & 1][warp - sub + w]);
     }
     __syncwarp();
     const float wanted = scale_for<C8>(amax);
@@ -459,7 +510,6 @@ __global__ void __launch_bounds__(kAppendThreads, 3) paged8_append_kernel(const 
       }
     }
   }
-  if (disorder && a.status != nullptr) *a.status = FA_STATUS_SLOT_ORDER;
 }
 
 int check_launch(const char* what, cudaError_t e) {
@@ -559,9 +609,10 @@ int launch_paged8_append(const fa_paged8_append_params& p, cudaStream_t stream) 
   while (a.warps > 1 && p.num_tokens <= 1024 && p.num_tokens * 2 * p.heads_kv * a.warps > 148 * 3 * kAppendWarps) a.warps /= 2;
   const int64_t tasks = (2 * p.heads_kv + kAppendWarps / a.warps - 1) / (kAppendWarps / a.warps);
   if (tasks > 65535) return set_error(FA_ERR_UNSUPPORTED, "append: too many heads");
-  // a CTA starts the runs of `range` tokens: one while the grid is small, up to a page's (at most 32) for prompts
+  // a CTA starts the runs of `range` tokens: one while the grid is small, up to a page's (at most 256) for prompts
   a.range = 1;
-  while (a.range < 32 && a.range < p.block_size && p.num_tokens * tasks / (2 * a.range) >= 592) a.range *= 2;
+  const bool wide = a.warps > 1;
+  while (a.range < (wide ? kAppendThreads : 32) && a.range < p.block_size && p.num_tokens * tasks / (2 * a.range) >= 592) a.range *= 2;
   const int64_t grid = (p.num_tokens + a.range - 1) / a.range;
   if (grid > INT32_MAX) return set_error(FA_ERR_UNSUPPORTED, "append: too many tokens");
   cudaLaunchAttribute attr;
@@ -573,14 +624,18 @@ int launch_paged8_append(const fa_paged8_append_params& p, cudaStream_t stream) 
   cfg.stream = stream;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  const bool e4m3 = p.cache_dtype == FA_CACHE_E4M3;
+  const bool e4m3 = p.cache_dtype == FA_CACHE_E4M3, fp16 = p.dtype == FA_F16;
   cudaError_t e;
-  if (p.dtype == FA_F16) {
-    e = e4m3 ? cudaLaunchKernelEx(&cfg, paged8_append_kernel<__half, CodeE4M3>, a)
-             : cudaLaunchKernelEx(&cfg, paged8_append_kernel<__half, CodeInt8>, a);
+  if (wide) {
+    if (fp16) e = e4m3 ? cudaLaunchKernelEx(&cfg, paged8_append_kernel<__half, CodeE4M3, true>, a)
+                       : cudaLaunchKernelEx(&cfg, paged8_append_kernel<__half, CodeInt8, true>, a);
+    else e = e4m3 ? cudaLaunchKernelEx(&cfg, paged8_append_kernel<__nv_bfloat16, CodeE4M3, true>, a)
+                  : cudaLaunchKernelEx(&cfg, paged8_append_kernel<__nv_bfloat16, CodeInt8, true>, a);
   } else {
-    e = e4m3 ? cudaLaunchKernelEx(&cfg, paged8_append_kernel<__nv_bfloat16, CodeE4M3>, a)
-             : cudaLaunchKernelEx(&cfg, paged8_append_kernel<__nv_bfloat16, CodeInt8>, a);
+    if (fp16) e = e4m3 ? cudaLaunchKernelEx(&cfg, paged8_append_kernel<__half, CodeE4M3, false>, a)
+                       : cudaLaunchKernelEx(&cfg, paged8_append_kernel<__half, CodeInt8, false>, a);
+    else e = e4m3 ? cudaLaunchKernelEx(&cfg, paged8_append_kernel<__nv_bfloat16, CodeE4M3, false>, a)
+                  : cudaLaunchKernelEx(&cfg, paged8_append_kernel<__nv_bfloat16, CodeInt8, false>, a);
   }
   return check_launch("append", e);
 }
