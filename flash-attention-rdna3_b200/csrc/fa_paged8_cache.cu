@@ -317,12 +317,11 @@ __global__ void __launch_bounds__(kAppendThreads, 3) paged8_append_kernel(const 
   __shared__ int count_s[kAppendWarps];
   [[maybe_unused]] const int tid = threadIdx.x;
   const int64_t t0 = (int64_t)blockIdx.x * a.range;
-  const int task = blockIdx.y * (kAppendWarps / a.warps) + warp / a.warps, sub = warp % a.warps;
+  const int task = blockIdx.y * (kAppendWarps / a.warps) + warp / a.warps, turn = warp % a.warps;
   const bool has_task = task < 2 * a.heads;
   const int kv = has_task ? task / a.heads : 0, head = has_task ? task % a.heads : 0;
   const int lanes = a.head_dim / 8, rows = 32 / lanes;  // lanes a row of 16-bit values, rows a load
   const int row = lane / lanes, col = lane % lanes;
-  const int chunk = kAppendLoads * rows * a.warps;      // tokens that the task's warps hold at once
   const char* src = reinterpret_cast<const char*>(a.src[kv]) + (head * a.src_sh[kv] + col * 8) * 2;
   uint8_t* cache = a.cache[kv] + head * a.c_sh[kv];
   const int lanes8 = a.head_dim / 16, rows8 = 32 / lanes8;
@@ -369,7 +368,13 @@ __global__ void __launch_bounds__(kAppendThreads, 3) paged8_append_kernel(const 
   }
   if (disorder && a.status != nullptr) *a.status = FA_STATUS_SLOT_ORDER;
 
-  for (int run = 0; run < runs; ++run) {
+  int parity = 0;
+  // Runs that a warp holds alone (a decode step's single tokens) are dealt to the task's warps, then all of them share each
+  // longer one.
+  for (int pass = 0; pass < (kWide ? 2 : 1); ++pass)
+  for (int run = kWide && pass == 0 ? turn : 0; run < runs; run += kWide && pass == 0 ? a.warps : 1) {
+    const int warps = kWide && pass == 1 ? a.warps : 1, sub = kWide && pass == 1 ? turn : 0;
+    const int chunk = kAppendLoads * rows * warps;  // tokens that these warps hold at once
     int i;
     int64_t slot;
     if constexpr (!kWide) {
@@ -411,6 +416,7 @@ __global__ void __launch_bounds__(kAppendThreads, 3) paged8_append_kernel(const 
       }
     }
     n = min(n, bs - offset);
+    if (kWide && (n > kAppendLoads * rows) != (pass == 1)) continue;
 
     // ---- largest magnitude of the run
     using P = typename Pair<T>::type;
@@ -438,17 +444,18 @@ __global__ void __launch_bounds__(kAppendThreads, 3) paged8_append_kernel(const 
       amax = 0.f;
       for (int j = first_j; j < end_j; j += rows) {
         const int l = (j - first_j) / rows;
-        if (l % (kAppendLoads * a.warps) >= kAppendLoads) continue;  // other warps' rows
+        if (l % (kAppendLoads * warps) >= kAppendLoads) continue;  // other warps' rows
         amax = fmaxf(amax, finite_amax8<T>(__ldg(reinterpret_cast<const uint4*>(mine + l * load_step))));
       }
     }
     amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));
     float* scale_at = a.scales[kv] + page * a.s_sb[kv] + head * a.s_sh[kv];
     const float old = offset > 0 ? *scale_at : 0.f;
-    if constexpr (kWide) {
-      if (lane == 0) part[run & 1][warp] = amax;
+    if (kWide && pass == 1) {
+      if (lane == 0) part[parity][warp] = amax;
       __syncthreads();  // also: every warp of the task has read the old scale
-      for (int w = 0; w < a.warps; ++w) amax = fmaxf(amax, part[run & 1][warp - sub + w]);
+      for (int w = 0; w < warps; ++w) amax = fmaxf(amax, part[parity][warp - sub + w]);
+      parity ^= 1;
     }
     __syncwarp();
     const float wanted = scale_for<C8>(amax);
@@ -461,7 +468,7 @@ __global__ void __launch_bounds__(kAppendThreads, 3) paged8_append_kernel(const 
     if (offset > 0 && scale != old) {
       const float ratio = __fdiv_rn(old, scale);
       const int r8 = lane / lanes8, c8 = lane % lanes8;
-      for (int j = sub * rows8 + r8; r8 < rows8 && j < offset; j += a.warps * rows8) {
+      for (int j = sub * rows8 + r8; r8 < rows8 && j < offset; j += warps * rows8) {
         uint4* at = reinterpret_cast<uint4*>(page_base + j * a.c_st[kv] + c8 * 16);
         uint4 v = *at;
         uint32_t* w = reinterpret_cast<uint32_t*>(&v);
@@ -606,7 +613,7 @@ int launch_paged8_append(const fa_paged8_append_params& p, cudaStream_t stream) 
   a.warps = 1;
   while (a.warps < kAppendWarps && a.warps * kAppendLoads * rows < p.block_size) a.warps *= 2;
   // (a few tokens are the single ones of a decode step: no more warps a task than there is room for at once)
-  while (a.warps > 1 && p.num_tokens <= 1024 && p.num_tokens * 2 * p.heads_kv * a.warps > 148 * 3 * kAppendWarps) a.warps /= 2;
+  while (a.warps > 1 && p.num_tokens <= 256 && p.num_tokens * 2 * p.heads_kv * a.warps > 148 * 3 * kAppendWarps) a.warps /= 2;
   const int64_t tasks = (2 * p.heads_kv + kAppendWarps / a.warps - 1) / (kAppendWarps / a.warps);
   if (tasks > 65535) return set_error(FA_ERR_UNSUPPORTED, "append: too many heads");
   // a CTA starts the runs of `range` tokens: one while the grid is small, up to a page's (at most 256) for prompts
