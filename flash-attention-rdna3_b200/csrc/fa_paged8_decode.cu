@@ -6,7 +6,7 @@
 // is read once for all query heads of its kv head, so the bound is HBM: 2 * head_dim bytes a token and kv head.
 //
 // One CTA an SM: a producer warp brings tiles of 64 KB (64, 32 or 16 tokens of 8 heads at head dims 64, 128, 256; of fewer
-// heads, accordingly more tokens) into a ring of three stages, one TMA box of up to 16 tokens x heads for each page and
+// heads, accordingly more tokens) into a ring of three stages, one TMA box of up to 128 rows (tokens x heads) for each page and
 // operand; eight compute warps own one kv head each (with fewer heads, a share of its tokens). Both products run on
 // m16n8k16 fp16 MMAs with tokens (then dimensions) as the 16 rows and up to 8 query heads as the 8 columns: a tensor
 // tile of 128 rows would be 15/16 empty at these group sizes. The codes are widened to fp16 in registers, exactly.
@@ -40,7 +40,7 @@ struct Args {
   int num_blocks, max_blocks, shift;
   int head_ctas, row_chunks;         // items of a request = groups of heads * chunks of query heads
   int head_shift;                    // log2 of the kv heads of a CTA
-  int box_shift, scale_shift;        // log2 of the tokens of a TMA box (at most 16), of a scale entry (at most 8)
+  int box_shift, scale_shift;        // log2 of the tokens of a TMA box, of a scale entry (at most 8)
   const void* q;
   int64_t q_sb, q_sh;
   const float* ks;
@@ -65,14 +65,15 @@ __host__ __device__ constexpr int item_rows(int heads_per_cta, int nt) { return 
 template <int D> struct Tile {
   static constexpr int kTokens = 4096 / D;            // tokens of a compute warp in a stage
   static constexpr int kMt = kTokens / 16;            // 16-token tiles
-  static constexpr int kRow = D < 128 ? D : 128;      // bytes of a row in shared memory (256 dimensions: two half tiles)
-  static constexpr int kHalves = D / kRow;
+  // A row of shared memory is 128 bytes: a token of one head, of two neighbouring heads of 64 dimensions, or half a token of
+  // 256 dimensions (TMA brings rows at one rate whatever their length: 64-byte rows would halve the bandwidth).
+  static constexpr int kPair = D == 64 ? 1 : 0;       // log2 of the heads in a row
+  static constexpr int kHalves = D == 256 ? 2 : 1;
 };
 
-// Rows of 128 (64) bytes lie in the 128-byte (64-byte) TMA swizzle: 16-byte chunk c of the row at offset x is chunk
-// c ^ (bits 7 .. 9 (7 .. 8) of x).
-template <int D>
-__device__ __forceinline__ uint32_t swizzle_of(uint32_t x) { return ((x >> 7) & (D == 64 ? 3u : 7u)) << 4; }
+// Rows lie in the 128-byte TMA swizzle: 16-byte chunk c of the row at offset x is chunk c ^ (bits 7 .. 9 of x).
+constexpr int kRow = 128;
+__device__ __forceinline__ uint32_t swizzle_of(uint32_t x) { return ((x >> 7) & 7u) << 4; }
 // token of an MMA row: a permutation (tokens are summed over) with which the K reads (four neighbouring chunks of the rows
 // r, r ^ 5) and the V reads (two chunks of four even or four odd rows) of a quarter warp touch every bank once
 __device__ __forceinline__ int token_of(int m) { return m ^ ((m & 1) << 2); }
@@ -167,7 +168,7 @@ template <typename C8, int D, int NT>
 __global__ void __launch_bounds__(kThreads, 1)
     paged8_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const Args a) {
   using T = Tile<D>;
-  constexpr int kTokens = T::kTokens, kMt = T::kMt, kJ = D / 64, kNm = D / 16, kRows = NT * 8, kRow = T::kRow;
+  constexpr int kTokens = T::kTokens, kMt = T::kMt, kJ = D / 64, kNm = D / 16, kRows = NT * 8;
   constexpr int kRoundTiles = NT == 1 ? 4 : 2, kCols = kRoundTiles * 16;  // columns of a merge round
   constexpr int kHalfBytes = kStageBytes / 2 / T::kHalves;
   extern __shared__ uint8_t smem_raw[];
@@ -260,7 +261,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp > kWarps) return;
     const int box = 1 << a.box_shift, boxes = span >> a.box_shift, in_page = (1 << a.shift) - 1;
     const int entries = (span >> a.scale_shift) << a.head_shift;
-    const uint32_t box_bytes = (uint32_t)(box << a.head_shift) * kRow;
+    const uint32_t box_bytes = (uint32_t)(box << (a.head_shift - T::kPair)) * kRow;
     auto page_at = [&](int pos) -> int {
       if (pos >= at.len) return -1;
       const int id = a.table[at.b * a.bt_sb + (pos >> a.shift) * a.bt_sk];
@@ -289,8 +290,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int c3 = id >= 0 ? id : a.num_blocks;
 #pragma unroll
         for (int h = 0; h < T::kHalves; ++h) {
-          tma_load_4d(kt + h * kHalfBytes + i * box_bytes, &k_map, &full_s[stage], h * 128, pos & in_page, head0, c3);
-          tma_load_4d(kt + kStageBytes / 2 + h * kHalfBytes + i * box_bytes, &v_map, &full_s[stage], h * 128, pos & in_page, head0, c3);
+          tma_load_4d(kt + h * kHalfBytes + i * box_bytes, &k_map, &full_s[stage], h * 128, pos & in_page, head0 >> T::kPair, c3);
+          tma_load_4d(kt + kStageBytes / 2 + h * kHalfBytes + i * box_bytes, &v_map, &full_s[stage], h * 128, pos & in_page, head0 >> T::kPair, c3);
         }
       }
       plain = __all_sync(0xffffffffu, plain);
@@ -350,18 +351,21 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int wh = warp >> (3 - a.head_shift), wt = warp & (warps_head - 1);
   float* merge = reinterpret_cast<float*>(smem + Smem<D, NT>::kRing + Smem<D, NT>::kScales);
   float2* stats = reinterpret_cast<float2*>(smem + Smem<D, NT>::kRing + Smem<D, NT>::kScales + Smem<D, NT>::kMerge);
-  // A box holds its tokens head by head, so token t (of the stage) of head h lies at row
-  // (t / box) * box * heads + h * box + t % box: 16 tokens further is 16 * heads rows, 8 tokens is 8 rows inside a box of
-  // 16 and 8 * heads rows otherwise, and the 8 tokens of a group differ by lane constants.
-  const int box = 1 << a.box_shift;
-  const uint32_t step16 = (uint32_t)(16 << a.head_shift) * kRow;
-  const uint32_t step8 = box == 16 ? 8u * kRow : (uint32_t)(8 << a.head_shift) * kRow;
-  auto lane_row = [&](int t) -> uint32_t {  // byte offset of token t < 8 of a group
-    return (uint32_t)(((t >> a.box_shift << a.box_shift) << a.head_shift) + wh * box + (t & (box - 1))) * kRow;
-  };
-  const uint32_t warp_base = smem_u32(smem) + wt * kMt * step16;
-  const uint32_t k_row = lane_row(token_of(g)), va_row = lane_row(token_of(2 * t4)), vb_row = lane_row(token_of(2 * t4 + 1));
-  const uint32_t k_swz = swizzle_of<D>(k_row), va_swz = swizzle_of<D>(va_row), vb_swz = swizzle_of<D>(vb_row);
+  // A box holds its tokens head by head (pair by pair), so token t (of the stage) of head h lies at row
+  // (t / box) * box * heads + h * box + t % box: a 16-token tile begins at tile_at[], 8 tokens further is 8 rows inside a
+  // box of 16 or more and 8 * heads rows otherwise, and the 8 tokens of a group differ by lane constants.
+  const int box = 1 << a.box_shift, layout_shift = a.head_shift - T::kPair;
+  const uint32_t step8 = box >= 16 ? 8u * kRow : (uint32_t)(8 << layout_shift) * kRow;
+  auto row_of = [&](int t) -> uint32_t { return (uint32_t)(((t >> a.box_shift << a.box_shift) << layout_shift) + (t & (box - 1))) * kRow; };
+  uint32_t tile_at[kMt];
+#pragma unroll
+  for (int mt = 0; mt < kMt; ++mt) tile_at[mt] = row_of(wt * kTokens + mt * 16);
+  const uint32_t head_at = smem_u32(smem) + (uint32_t)((wh >> T::kPair) * box) * kRow;
+  const uint32_t k_row = row_of(token_of(g)), va_row = row_of(token_of(2 * t4)), vb_row = row_of(token_of(2 * t4 + 1));
+  // (the swizzle follows the address: the head's rows count too where a box has fewer than 8 tokens)
+  const uint32_t head_rows = (uint32_t)((wh >> T::kPair) * box) * kRow;
+  const uint32_t k_swz = swizzle_of(k_row + head_rows), va_swz = swizzle_of(va_row + head_rows), vb_swz = swizzle_of(vb_row + head_rows);
+  const uint32_t half_row = (wh & T::kPair) * 4;  // first chunk of the head in its row
   const uint32_t scale8 = (uint32_t)((8 >> a.scale_shift) << a.head_shift) * 4;
   const uint32_t scale_base = smem_u32(smem) + Smem<D, NT>::kRing + wt * kMt * 2 * scale8 +
                               (((token_of(g) >> a.scale_shift) << a.head_shift) + wh) * 4;
@@ -452,30 +456,40 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     wait_for(&full_s[stage], parity, lost, a.status);
     const bool plain = plain_s[stage] != 0;
-    const uint32_t kt = warp_base + stage * kStageBytes, vt = kt + kStageBytes / 2;
+    const uint32_t kt = head_at + stage * kStageBytes, vt = kt + kStageBytes / 2;
     const uint32_t st = scale_base + stage * Smem<D, NT>::kScaleStage;
     const int left = at.len - (at.step * span + wt * kTokens);  // tokens of the context from this tile's first on
     // ---- scores: rows are tokens, columns query heads
     float s[kMt][NT][4];
 #pragma unroll
     for (int mt = 0; mt < kMt; ++mt) {
+      // (256 dimensions are sixteen products in a row with one 16-token tile to work on: four sums instead of one)
+      constexpr int kSums = D == 256 ? 4 : 1;
+      float sums[kSums][NT][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int x = 0; x < kSums; ++x)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) s[mt][nt][c] = 0.f;
-      const uint32_t row = kt + mt * step16 + k_row;
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) sums[x][nt][c] = 0.f;
+      const uint32_t row = kt + tile_at[mt] + k_row;
 #pragma unroll
       for (int j = 0; j < kJ; ++j) {
-        const uint32_t chunk = ((uint32_t)((t4 + 4 * (j & 1)) << 4) ^ k_swz) + (j >> 1) * kHalfBytes;
+        const uint32_t chunk = (((half_row + t4 + 4 * (j & 1)) << 4) ^ k_swz) + (j >> 1) * kHalfBytes;
         const uint4 ka = lds128(row + chunk), kb = lds128(row + step8 + chunk);
         const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const uint32_t a0 = C8::lo(wa[i]), a1 = C8::lo(wb[i]), a2 = C8::hi(wa[i]), a3 = C8::hi(wb[i]);
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma(s[mt][nt], a0, a1, a2, a3, qf[nt][j * 4 + i][0], qf[nt][j * 4 + i][1]);
+          for (int nt = 0; nt < NT; ++nt) mma(sums[i % kSums][nt], a0, a1, a2, a3, qf[nt][j * 4 + i][0], qf[nt][j * 4 + i][1]);
         }
       }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          s[mt][nt][c] = kSums == 1 ? sums[0][nt][c] : (sums[0][nt][c] + sums[1 % kSums][nt][c]) + (sums[2 % kSums][nt][c] + sums[3 % kSums][nt][c]);
     }
     // ---- Scales and mask. m is a reference, not the maximum: it moves (with everything summed so far) only when a score
     // passes it by more than 2^kSlack, so most tiles need no reduction over the warp. The products with V take p * vs
@@ -584,9 +598,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       // rows behind the context may hold anything, NaN among it: zeros there
       const int r = mt * 16 + token_of(2 * t4), r2 = mt * 16 + token_of(2 * t4 + 1);
-      const uint32_t row_a = vt + mt * step16 + va_row, row_b = vt + mt * step16 + vb_row;
+      const uint32_t row_a = vt + tile_at[mt] + va_row, row_b = vt + tile_at[mt] + vb_row;
       if constexpr (D == 64) {
-        const uint32_t ca = ((uint32_t)((g >> 1) << 4) ^ va_swz) + (g & 1) * 8, cb = ((uint32_t)((g >> 1) << 4) ^ vb_swz) + (g & 1) * 8;
+        const uint32_t ca = (((half_row + (g >> 1)) << 4) ^ va_swz) + (g & 1) * 8, cb = (((half_row + (g >> 1)) << 4) ^ vb_swz) + (g & 1) * 8;
         uint2 va = lds64(row_a + ca), vb = lds64(row_b + cb);
         uint2 vc = lds64(row_a + step8 + ca), vd = lds64(row_b + step8 + cb);
         if (!plain) {
@@ -881,10 +895,14 @@ Shape shape_of(const fa_paged8_params& p) {
   const int group = p.heads_q / p.heads_kv;
   s.head_shift = 3;
   while (p.heads_kv % (1 << s.head_shift)) --s.head_shift;
+  // Two neighbouring heads of 64 dimensions make a row (see Tile); where they are not neighbours, and for fewer dimensions,
+  // rows are padded to 128 by the tensor map (which reads nothing for the padding).
+  const bool pairs = p.head_dim == 64 && s.head_shift > 0 && p.k_strides[2] == 64 && p.v_strides[2] == 64;
+  s.D = pairs ? 64 : p.head_dim <= 128 ? 128 : 256;
+  // A box is up to 128 rows (16 KB) of a page: boxes of 16 rows reach 60 % of the rate of boxes of 64 and more.
+  const int layout_shift = s.head_shift - (pairs ? 1 : 0);
   s.box_shift = 0;
-  while (s.box_shift < 4 && (2 << s.box_shift) <= p.block_size) ++s.box_shift;
-  // (a box of one 64-byte row would not start on the 128 bytes that TMA asks for: such rows are padded to 128)
-  s.D = p.head_dim <= 64 && s.head_shift + s.box_shift > 0 ? 64 : p.head_dim <= 128 ? 128 : 256;
+  while ((2 << s.box_shift) <= p.block_size && (2 << s.box_shift << layout_shift) <= 128) ++s.box_shift;
   s.nt = group > 8 && s.D <= 128 ? 2 : 1;
   s.row_chunks = (group + s.nt * 8 - 1) / (s.nt * 8);
   return s;
@@ -916,13 +934,14 @@ int cta_count() {
 int make_cache_map(CUtensorMap* map, const void* ptr, const fa_paged8_params& p, const int64_t (&st)[4], const Shape& s) {
   TensorMapEncodeFn enc = tensor_map_encoder();
   if (enc == nullptr) return set_error(FA_ERR_DEVICE, "cuTensorMapEncodeTiled is not available from this driver");
-  const cuuint64_t dims[4] = {(cuuint64_t)p.head_dim, (cuuint64_t)p.block_size, (cuuint64_t)p.heads_kv, (cuuint64_t)p.num_blocks};
+  const int pair = s.D == 64 ? 1 : 0, heads = p.heads_kv >> pair;
+  const cuuint64_t dims[4] = {(cuuint64_t)p.head_dim << pair, (cuuint64_t)p.block_size, (cuuint64_t)heads, (cuuint64_t)p.num_blocks};
   auto stride = [&](int64_t x, int64_t n) { return (cuuint64_t)(n > 1 ? x : 256); };  // a size-1 dimension never advances
-  const cuuint64_t strides[3] = {stride(st[1], p.block_size), stride(st[2], p.heads_kv), stride(st[0], p.num_blocks)};
-  const cuuint32_t box[4] = {(cuuint32_t)(s.D < 128 ? s.D : 128), 1u << s.box_shift, 1u << s.head_shift, 1};
+  const cuuint64_t strides[3] = {stride(st[1], p.block_size), stride(st[2] << pair, heads), stride(st[0], p.num_blocks)};
+  const cuuint32_t box[4] = {kRow, 1u << s.box_shift, 1u << (s.head_shift - pair), 1};
   const cuuint32_t one[4] = {1, 1, 1, 1};
   const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(ptr), dims, strides, box, one,
-                         CU_TENSOR_MAP_INTERLEAVE_NONE, s.D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return set_error(FA_ERR_UNSUPPORTED, "8-bit paged decode: no tensor map for this cache layout (code %d)", (int)r);
   return 0;

@@ -320,7 +320,9 @@ def check_decode(args, **kw):
     ([1], 1, 1, 64, 16), ([256], 8, 8, 128, 16), ([1000, 3], 32, 8, 128, 16), ([77, 0, 300], 4, 2, 64, 8),
     ([129, 128, 127], 16, 1, 128, 32), ([513], 10, 2, 256, 64), ([40, 900], 24, 8, 16, 16), ([65, 31], 15, 3, 32, 4),
     ([700, 1, 64], 32, 2, 64, 1), ([333], 12, 12, 128, 128), ([50, 2000], 20, 4, 128, 256), ([257], 33, 1, 256, 16),
-    ([5, 6, 7, 8], 64, 4, 128, 2), ([1500], 40, 1, 128, 16), ([90, 91], 48, 16, 64, 16)])
+    ([5, 6, 7, 8], 64, 4, 128, 2), ([1500], 40, 1, 128, 16), ([90, 91], 48, 16, 64, 16), ([333, 70], 6, 3, 64, 32),
+    ([500, 129], 12, 2, 64, 2), ([260, 7], 8, 4, 64, 4), ([300, 5], 4, 2, 128, 64), ([300, 1], 3, 1, 256, 256),
+    ([200, 130], 4, 1, 32, 128), ([77], 2, 2, 16, 1)])
 def test_decode(cache, dtype, lens, heads_q, heads_kv, dim, bs):
     check_decode(decode_case(len(lens) * 7 + dim, lens, heads_q, heads_kv, dim, bs, dtype, cache))
 
@@ -405,20 +407,23 @@ def test_decode_nan_stays_in_its_row():
     assert torch.equal(got[rest], clean[rest])
 
 
+@pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("cache", CACHES)
-def test_decode_strided(cache):
-    args = decode_case(12, [100, 333], 8, 4, 64, 16, torch.float16, cache)
+def test_decode_strided(cache, dim):
+    """Every layout against the oracle; at 128 dimensions all of them take the same way, bit for bit (at 64 neighbouring
+    heads are read in pairs, heads that are not neighbours one by one, and the sums are split differently)."""
+    args = decode_case(12, [100, 333], 8, 4, dim, 16, torch.float16, cache)
     q, k, v, ks, vs, table, lens = args
     both = torch.cat((k.view(torch.uint8), v.view(torch.uint8)), -1).view(cache)          # K and V side by side
     major = v.view(torch.uint8).transpose(1, 2).contiguous().transpose(1, 2).view(cache)   # head-major pages
     qkv = torch.cat((q, q, q), 1)
-    want = fa_b200.flash_attention_decode_paged_8bit(*args)
+    want = check_decode(args)
     scales = torch.stack((ks, vs), 2)
-    for kk, vv in ((both[..., :64], both[..., 64:]), (k, major), (both[..., :64], major)):
-        got = fa_b200.flash_attention_decode_paged_8bit(qkv[:, 8:16], kk, vv, scales[..., 0], scales[..., 1],
-                                                        table.T.contiguous().T, torch.stack((lens, lens), 1)[:, 1])
-        assert torch.equal(got, want)
-    odd = torch.zeros(2, 8, 65, dtype=q.dtype, device="cuda")[..., 1:]
+    for kk, vv in ((both[..., :dim], both[..., dim:]), (k, major), (both[..., :dim], major)):
+        got = check_decode([qkv[:, 8:16], kk, vv, scales[..., 0], scales[..., 1], table.T.contiguous().T,
+                            torch.stack((lens, lens), 1)[:, 1]])
+        assert dim == 64 or torch.equal(got, want)
+    odd = torch.zeros(2, 8, dim + 1, dtype=q.dtype, device="cuda")[..., 1:]
     odd.copy_(q)
     assert torch.equal(fa_b200.flash_attention_decode_paged_8bit(odd, *args[1:]), want)
 
