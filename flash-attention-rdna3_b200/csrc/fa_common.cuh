@@ -400,5 +400,6 @@ int launch_paged8_append(const fa_paged8_append_params& p, cudaStream_t stream);
 int launch_decode_paged8(const fa_paged8_params& p, cudaStream_t stream);         // fa_paged8_decode.cu
 int64_t paged8_workspace_bytes(const fa_paged8_params& p);
 void set_decode_fault_injection(uint32_t poll_limit, int skip_tile);
+void take_decode_fault_injection(uint32_t* poll_limit, int* skip_tile);  // what the next launch is to use; then the defaults
 
 }  // namespace fa

@@ -1095,10 +1095,7 @@ thread_local uint32_t g_fault_poll_limit = 0;
 thread_local int g_fault_skip_tile = -1;
 
 void take_fault_injection(DecArgs* a) {
-  a->poll_limit = g_fault_poll_limit ? g_fault_poll_limit : kWaitPollLimit;
-  a->skip_tile = g_fault_skip_tile;
-  g_fault_poll_limit = 0;
-  g_fault_skip_tile = -1;
+  take_decode_fault_injection(&a->poll_limit, &a->skip_tile);
 }
 
 }  // namespace
@@ -1286,6 +1283,13 @@ int launch_paged_tc(const fa_paged_params& p, cudaStream_t stream) {
 }
 
 PROF_DEFINE_READER(fa_debug_read_prof_decode)
+
+void take_decode_fault_injection(uint32_t* poll_limit, int* skip_tile) {
+  *poll_limit = g_fault_poll_limit ? g_fault_poll_limit : kWaitPollLimit;
+  *skip_tile = g_fault_skip_tile;
+  g_fault_poll_limit = 0;
+  g_fault_skip_tile = -1;
+}
 
 void set_decode_fault_injection(uint32_t poll_limit, int skip_tile) {
   g_fault_poll_limit = poll_limit;

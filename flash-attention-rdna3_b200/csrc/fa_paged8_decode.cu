@@ -54,6 +54,8 @@ struct Args {
   int64_t o_sb, o_sh;
   float scale_log2;
   int32_t* status;
+  uint32_t poll_limit;  // polls of a barrier wait before it is given up
+  int skip_unit;        // test hook: unit of every CTA whose tiles are not brought (-1: none)
   int4* cuts;        // for every CTA: request, item, first CTA and number of CTAs of the item that its stretch begins inside
   float* part_stat;  // (2 * CTAs, rows of a CTA, 2): m, l
   float* part_o;     // (2 * CTAs, rows of a CTA, D)
@@ -157,11 +159,12 @@ template <int D, int NT> struct Smem {
   static constexpr int kBytes = kRing + kScales + kMerge + kStats + 1024;  // the ring is moved to a 1024-byte boundary
 };
 
-// Waits for a phase; a wait that runs out is recorded, and later ones are not begun.
-__device__ __forceinline__ void wait_for(uint64_t* bar, uint32_t parity, bool& lost, int32_t* status) {
-  if (lost || mbar_wait(bar, parity)) return;
-  lost = true;
-  if (status != nullptr) *status = 1;
+// Waits for a phase, all lanes of a warp alike; a wait that runs out is recorded, and later ones are not begun.
+__device__ __forceinline__ void wait_for(uint64_t* bar, uint32_t parity, bool& lost, const Args& a) {
+  if (lost) return;
+  const bool done = mbar_wait_limit(bar, parity, a.poll_limit);
+  lost = __any_sync(0xffffffffu, !done);
+  if (lost && a.status != nullptr) *a.status = 1;
 }
 
 template <typename C8, int D, int NT>
@@ -273,8 +276,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int stage = 0, issued = 0;
     uint32_t parity = 1;
     for (; issued < units; ++issued) {
-      if (issued >= kStages) wait_for(&empty_s[stage], parity, lost, a.status);
-      lost = __any_sync(0xffffffffu, lost);
+      if (issued >= kStages) wait_for(&empty_s[stage], parity, lost, a);
       if (lost) break;
       const int head0 = (at.item / a.row_chunks) << a.head_shift, pos0 = at.step * span;
       uint8_t* kt = smem + stage * kStageBytes;
@@ -283,7 +285,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(&full_s[stage])), "n"(kStageBytes) : "memory");
       __syncwarp();
       bool plain = true;
-      for (int i = lane; i < boxes; i += 32) {
+      for (int i = lane; i < boxes && issued != a.skip_unit; i += 32) {
         const int pos = pos0 + i * box, id = i < 32 ? page : page_at(pos);
         plain = plain && id >= 0 && pos + box <= at.len;
         // tokens behind the context and pages out of range: a page behind the last one, which reads as zeros
@@ -324,8 +326,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     if (lost) {  // copies on the way land before the CTA leaves
-      bool ignored = false;
-      for (int i = max(0, issued - kStages); i < issued; ++i) wait_for(&full_s[i % kStages], (i / kStages) & 1, ignored, a.status);
+      for (int i = max(0, issued - kStages); i < issued; ++i) {
+        bool gone = false;
+        wait_for(&full_s[i % kStages], (i / kStages) & 1, gone, a);
+      }
     }
     return;
   }
@@ -454,11 +458,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
 
-    wait_for(&full_s[stage], parity, lost, a.status);
+    wait_for(&full_s[stage], parity, lost, a);
     const bool plain = plain_s[stage] != 0;
     const uint32_t kt = head_at + stage * kStageBytes, vt = kt + kStageBytes / 2;
     const uint32_t st = scale_base + stage * Smem<D, NT>::kScaleStage;
     const int left = at.len - (at.step * span + wt * kTokens);  // tokens of the context from this tile's first on
+    if (!lost) {
     // ---- scores: rows are tokens, columns query heads
     float s[kMt][NT][4];
 #pragma unroll
@@ -630,8 +635,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
     }
+    } else {  // the tile never came: this part of the item hands in nothing
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        m[nt][0] = m[nt][1] = kNegInf;
+        l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+        for (int i = 0; i < kNm; ++i)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) o[nt][i][c] = 0.f;
+      }
+    }
     __syncwarp();  // every lane is done with the stage
-    if (lane == 0) mbar_arrive(&empty_s[stage]);
+    // A warp that has lost a wait hands no stage back: the loading warp then stops at its own bounded wait, and no barrier
+    // is armed again whose phase is still open (arriving there once more is undefined).
+    if (lane == 0 && !lost) mbar_arrive(&empty_s[stage]);
     if (++stage == kStages) {
       stage = 0;
       parity ^= 1;
@@ -1040,6 +1058,7 @@ int launch_decode_paged8(const fa_paged8_params& p, cudaStream_t stream) {
   a.o_sh = p.o_strides[1];
   a.scale_log2 = p.softmax_scale * kLog2e;
   a.status = p.status;
+  take_decode_fault_injection(&a.poll_limit, &a.skip_unit);
   a.cuts = static_cast<int4*>(p.workspace);
   a.part_stat = reinterpret_cast<float*>(a.cuts + ctas);
   a.part_o = a.part_stat + (int64_t)2 * ctas * item_rows(1 << s.head_shift, s.nt) * 2;

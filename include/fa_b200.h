@@ -388,7 +388,7 @@ FA_API int32_t fa_paged_plan(const fa_paged_plan_params* p, void* stream);
 FA_API int32_t fa_paged8_append(const fa_paged8_append_params* p, void* stream);
 FA_API int32_t fa_decode_paged8(const fa_paged8_params* p, void* stream);
 
-/* Test hook, no counterpart in the reference: makes the NEXT tensor-core decode launch (dense or paged) of the
+/* Test hook, no counterpart in the reference: makes the NEXT tensor-core decode launch (dense, paged or paged 8-bit) of the
    calling thread use `poll_limit` polls per barrier wait (0 = the default, about a second) and leave out the
    loads of tile `skip_tile` of every CTA (-1 = none), so that a wait runs out, the kernel leaves through its
    normal exit and the status word is set. Nothing faults and nothing hangs. */

@@ -644,3 +644,21 @@ def test_captured_behind_copies_and_joined_streams():
             torch.cuda.synchronize()
             for a, b in zip(got, ref):
                 assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("skip", [0, 4])
+def test_decode_lost_wait_sets_the_status_word(skip):
+    """The loading warp leaves a unit out, so that bounded waits run out on both sides; the kernel ends by itself, what it
+    could not read counts as nothing, and the next call is right."""
+    from fa_b200 import _lib
+
+    args = decode_case(24, [30000], 32, 8, 128, 16, torch.float16, E4M3)
+    check_decode(args)
+    fa_b200.check_status()
+    _lib.load().fa_test_decode_fault(1 << 12, skip)
+    got = fa_b200.flash_attention_decode_paged_8bit(*args)
+    with pytest.raises(RuntimeError, match="wait timeout"):
+        fa_b200.check_status()
+    assert torch.isfinite(got).all()
+    check_decode(args)
+    fa_b200.check_status()
