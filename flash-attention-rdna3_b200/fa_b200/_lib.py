@@ -20,7 +20,7 @@ FA_WS_FWD_P = 7
 FA_WS_PAGED8 = 8
 FA_CACHE_E4M3, FA_CACHE_INT8 = 0, 1
 FA_PLAN_MAX_BATCH = 8192
-FA_STATUS_SLOT_ORDER = 101
+FA_STATUS_SLOT_ORDER = 901
 ABI_VERSION = 3
 
 I64x4 = C.c_int64 * 4

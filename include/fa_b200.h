@@ -277,7 +277,7 @@ typedef struct fa_paged8_append_params {
   const int64_t* slot_mapping; int64_t slot_stride;
   int32_t* status;                /* may be NULL */
 } fa_paged8_append_params;
-#define FA_STATUS_SLOT_ORDER 101
+#define FA_STATUS_SLOT_ORDER 901
 
 /* Decode attention over the 8-bit cache: q, out (batch, heads_q, head_dim) fp16 or bf16, the rest as in
    fa_paged_params (context lengths are clamped to the table, page ids out of range contribute nothing, an empty context
