@@ -662,3 +662,52 @@ def test_decode_lost_wait_sets_the_status_word(skip):
     assert torch.isfinite(got).all()
     check_decode(args)
     fa_b200.check_status()
+
+
+def test_plan_of_the_largest_batches():
+    check_plan(random_plan(41, 8192, 16, 24, 40, 60000), 16)
+    args = random_plan(42, 300, 16, 400, 3000, 40000, ends=0.1, pad=5000)
+    assert args[5] > 350000
+    check_plan(args, 16)
+    check_plan(random_plan(43, 300, 16, 400, 3000, 40000, ends=0.1), 16, inplace=True)
+
+
+@pytest.mark.parametrize("cache", CACHES)
+def test_pages_of_a_thousand_tokens(cache):
+    """Runs that are longer than what a CTA looks at, and boxes that are a part of a page."""
+    bs, heads, dim = 1024, 2, 64
+    k, ks = filled_cache(1, 5, bs, heads, dim, cache)
+    v, vs = filled_cache(2, 5, bs, heads, dim, cache)
+    slots = runs_to_slots([(3, 100, 924), (0, 0, 1024), (None, 0, 1), (4, 0, 333), (2, 1023, 1)], bs)
+    n = slots.numel()
+    check_append(inputs(3, n, heads, dim, torch.float16), inputs(4, n, heads, dim, torch.bfloat16).half(), k, v, ks, vs, slots)
+    check_decode(decode_case(25, [2500, 1024, 1025, 3], 8, 2, 64, 1024, torch.bfloat16, cache))
+    check_decode(decode_case(26, [1500, 77], 4, 1, 256, 512, torch.float16, cache))
+
+
+def test_decode_one_kv_head_under_many_query_heads():
+    check_decode(decode_case(27, [600, 90], 128, 1, 128, 16, torch.bfloat16, E4M3))
+    check_decode(decode_case(28, [300], 71, 1, 256, 32, torch.float16, torch.int8))
+
+
+def test_a_compiled_step_of_all_three():
+    """plan, append and decode inside one compiled function, with the state that they change in place."""
+    heads, dim, bs = 2, 64, 16
+
+    def step(lens, new, table, free, count, key, value, k, v, ks, vs, q):
+        slots, cu, lens, count = fa_b200.paged_kv_plan(lens, new, table, free, count, 40, bs)
+        fa_b200.paged_kv_append(key, value, k, v, ks, vs, slots)
+        return fa_b200.flash_attention_decode_paged_8bit(q, k, v, ks, vs, table, lens), slots, cu, lens, count
+
+    def state():
+        k, ks = filled_cache(1, 12, bs, heads, dim, torch.int8)
+        v, vs = filled_cache(2, 12, bs, heads, dim, torch.int8)
+        x = inputs(3, 40, heads, dim, torch.float16)
+        return [ints([0, 0]), ints([30, 7]), torch.full((2, 5), -1, dtype=torch.int32, device="cuda"),
+                torch.arange(12, dtype=torch.int32, device="cuda"), ints([12]), x, -x, k, v, ks, vs,
+                inputs(4, 2 * 8, 1, dim, torch.float16).view(2, 8, dim)]
+
+    a, b = state(), state()
+    want, got = step(*a), torch.compile(step, backend="aot_eager", fullgraph=True)(*b)
+    assert all(torch.equal(x, y) for x, y in zip(want, got))
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
