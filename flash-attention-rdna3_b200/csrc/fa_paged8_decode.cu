@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr int kHalfBytes = kStageBytes / 2 / T::kHalves;
   extern __shared__ uint8_t smem_raw[];
   __shared__ int64_t scan_s[kWarps];
-  __shared__ int64_t start_s[2];
+  __shared__ int64_t start_s[3];
   __shared__ __align__(8) uint64_t full_s[kStages], empty_s[kStages];
   __shared__ int plain_s[kStages];  // whether every token of the stage is there
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -206,8 +206,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   Stretches cut_line;
   {
     const int per = (a.batch + kWarps * 32 - 1) / (kWarps * 32), b0 = min(tid * per, a.batch), b1 = min(b0 + per, a.batch);
-    int64_t mine = 0;
-    for (int b = b0; b < b1; ++b) mine += (int64_t)((clamped_len(a, b) + span - 1) / span) * items;
+    const int len0 = b0 < b1 ? clamped_len(a, b0) : 0;  // (the only one of this thread up to 256 requests)
+    int64_t mine = (int64_t)((len0 + span - 1) / span) * items;
+    for (int b = b0 + 1; b < b1; ++b) mine += (int64_t)((clamped_len(a, b) + span - 1) / span) * items;
     int64_t sum = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -237,10 +238,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     int64_t at = sum - mine;
     if (u_begin < u_end && at <= u_begin && u_begin < sum) {
       for (int b = b0; b < b1; ++b) {
-        const int64_t n = (int64_t)((clamped_len(a, b) + span - 1) / span) * items;
+        const int len = b == b0 ? len0 : clamped_len(a, b);
+        const int64_t n = (int64_t)((len + span - 1) / span) * items;
         if (at <= u_begin && u_begin < at + n) {
           start_s[0] = b;
           start_s[1] = at;
+          start_s[2] = len;
         }
         at += n;
       }
@@ -251,7 +254,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   Cursor at;
   if (units > 0) {
     at.b = (int)start_s[0];
-    at.enter(a, span);
+    at.len = (int)start_s[2];
+    at.steps = (at.len + span - 1) / span;
     const int64_t rest = u_begin - start_s[1];
     if (rest < INT32_MAX) {
       at.item = (int)rest / at.steps;
@@ -271,14 +275,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int box = 1 << a.box_shift, boxes = span >> a.box_shift, in_page = (1 << a.shift) - 1;
     const int entries = (span >> a.scale_shift) << a.head_shift;
     const uint32_t box_bytes = (uint32_t)(box << (a.head_shift - T::kPair)) * kRow;
-    auto page_at = [&](int pos) -> int {
-      if (pos >= at.len) return -1;
-      const int id = a.table[at.b * a.bt_sb + (pos >> a.shift) * a.bt_sk];
+    auto page_at = [&](const Cursor& c, int pos) -> int {
+      if (pos >= c.len) return -1;
+      const int id = a.table[c.b * a.bt_sb + (pos >> a.shift) * a.bt_sk];
       return id >= 0 && id < a.num_blocks ? id : -1;
     };
-    auto fetch = [&]() -> int { return lane < boxes ? page_at(at.step * span + lane * box) : -1; };
+    auto fetch = [&](const Cursor& c) -> int { return lane < boxes ? page_at(c, c.step * span + lane * box) : -1; };
     int page = -1;
-    if (units > 0) page = fetch();
+    if (units > 0) page = fetch(at);
     int stage = 0, issued = 0;
     uint32_t parity = 1;
     for (; issued < units; ++issued) {
@@ -292,7 +296,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       bool plain = true;
       for (int i = lane; i < boxes && issued != a.skip_unit; i += 32) {
-        const int pos = pos0 + i * box, id = i < 32 ? page : page_at(pos);
+        const int pos = pos0 + i * box, id = i < 32 ? page : page_at(at, pos);
         plain = plain && id >= 0 && pos + box <= at.len;
         // tokens behind the context and pages out of range: a page behind the last one, which reads as zeros
         const int c3 = id >= 0 ? id : a.num_blocks;
@@ -306,7 +310,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int e0 = 0; e0 < entries; e0 += 32) {
         const int e = e0 + lane, pos = pos0 + ((e >> a.head_shift) << a.scale_shift);
         int id = __shfl_sync(0xffffffffu, page, ((pos - pos0) >> a.box_shift) & 31);
-        if (boxes > 32) id = page_at(pos);
+        if (boxes > 32) id = page_at(at, pos);
         if (e >= entries) continue;
         const uint32_t k_to = st + e * 4, v_to = k_to + entries * 4;
         const int head = head0 + (e & (heads_cta - 1));
@@ -324,7 +328,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&full_s[stage])) : "memory");
       if (issued + 1 < units) {
         at.advance(a, span, items);
-        page = fetch();
+        page = fetch(at);
       }
       if (++stage == kStages) {
         stage = 0;
