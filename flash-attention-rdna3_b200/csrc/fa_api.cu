@@ -252,8 +252,8 @@ int check_cache8(int dtype, int cache_dtype, int heads_kv, int head_dim, int num
     return fa::set_error(FA_ERR_INVALID_ARGUMENT, "8-bit cache: the cache must be float8_e4m3fn or int8");
   if (heads_kv <= 0 || num_blocks <= 0 || block_size <= 0 || (block_size & (block_size - 1)))
     return fa::set_error(FA_ERR_INVALID_ARGUMENT, "8-bit cache: heads and blocks must be positive, the block size a power of two");
-  if (head_dim <= 0 || head_dim > 256 || head_dim % 16)
-    return fa::set_error(FA_ERR_UNSUPPORTED, "8-bit cache: head_dim must be a multiple of 16 up to 256, got %d", head_dim);
+  if (head_dim < 16 || head_dim > 256 || (head_dim & (head_dim - 1)))
+    return fa::set_error(FA_ERR_UNSUPPORTED, "8-bit cache: head_dim must be 16, 32, 64, 128 or 256, got %d", head_dim);
   if (!cache_rows_ok(k, ks, num_blocks, block_size, heads_kv) || !cache_rows_ok(v, vs, num_blocks, block_size, heads_kv))
     return fa::set_error(FA_ERR_UNSUPPORTED, "8-bit cache: caches need unit inner stride and rows on 16-byte boundaries");
   return 0;

@@ -225,7 +225,7 @@ typedef struct fa_paged_params {
 /* ---- paged KV cache held in 8 bits (no counterpart in the reference, whose caches are 16-bit and filled by the caller) ----
 
    Caches (num_blocks, block_size, heads_kv, head_dim) of fa_cache_dtype with unit inner stride, rows on 16-byte
-   boundaries and head_dim a multiple of 16 up to 256; block_size a power of two. One fp32 scale for each block and kv
+   boundaries and head_dim 16, 32, 64, 128 or 256; block_size a power of two. One fp32 scale for each block and kv
    head, (num_blocks, heads_kv): a stored code c stands for c * scale. The three entry points below are what a server
    runs in every step: fa_paged_plan once, then fa_paged8_append and fa_decode_paged8 in every layer. */
 enum fa_cache_dtype { FA_CACHE_E4M3 = 0, FA_CACHE_INT8 = 1 };

@@ -148,7 +148,7 @@ def test_c_entries_refuse_without_a_gpu():
     append = dict(dtype=_lib.FA_F16, cache_dtype=0, heads_kv=2, head_dim=64, num_blocks=4, block_size=16, num_tokens=1,
                   key=at, key_strides=(128, 64, 1), value=at, value_strides=(128, 64, 1), k_cache=at, k_strides=strides,
                   v_cache=at, v_strides=strides, k_scales=at, v_scales=at, slot_mapping=at)
-    for bad in (dict(dtype=_lib.FA_F32), dict(cache_dtype=2), dict(head_dim=72), dict(head_dim=272), dict(block_size=24),
+    for bad in (dict(dtype=_lib.FA_F32), dict(cache_dtype=2), dict(head_dim=72), dict(head_dim=96), dict(head_dim=512), dict(block_size=24),
                 dict(k_cache=at + 8), dict(v_strides=(2048, 128, 64, 2)), dict(k_strides=(2048, 128, 72, 1)),
                 dict(k_strides=(0, 128, 64, 1)), dict(key=at + 8), dict(key_strides=(128, 60, 1)), dict(v_scales=None)):
         assert lib.fa_paged8_append(ctypes.byref(_lib.Paged8AppendParams(**{**append, **bad})), None) < 0, bad
