@@ -152,7 +152,8 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanArgs
     back_sum += tb;
     need_sum += tn;
   }
-  const int available = saturated(count + back_sum);
+  // (below the value that running sums stop at, so that a request behind 2^31 needed pages is never taken for served)
+  const int available = (int)min(count + back_sum, (int64_t)INT32_MAX - 1);
   __syncthreads();
   for (int b = tid; b < a.batch; b += threads)
     if (state[b] == kNeedsPages && need_end[b] > available) state[b] = kUnserved;
@@ -371,7 +372,6 @@ __global__ void __launch_bounds__(kAppendThreads, 3) paged8_append_kernel(const 
     }
     __syncthreads();
     for (int w = 0; w < kAppendWarps; ++w) runs += count_s[w];
-
   }
   if (disorder && a.status != nullptr) *a.status = FA_STATUS_SLOT_ORDER;
 
