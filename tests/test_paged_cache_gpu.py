@@ -383,6 +383,31 @@ def test_decode_scales_of_every_size():
     check_decode(args)
 
 
+@pytest.mark.parametrize("heads_q, heads_kv, dim", [(8, 2, 64), (32, 2, 64), (16, 8, 128), (12, 1, 128), (5, 1, 256)])
+@pytest.mark.parametrize("first", [True, False])
+def test_decode_large_value_scales_under_small_probabilities(heads_q, heads_kv, dim, first):
+    """Values many powers of two larger than the others, in pages that the softmax leaves next to nothing of: the answer
+    is that of the others. The large ones come in front of them or behind, and one row in two has them on top instead."""
+    args = decode_case(12, [300, 5000, 64], heads_q, heads_kv, dim, 16, torch.bfloat16, E4M3)
+    q, k, v, ks, vs, table, lens = args
+    ks.fill_(2.0 ** -6)
+    k.copy_((torch.randn(k.shape, generator=gen(4)) * 0.1).to(E4M3))
+    q.copy_(torch.randn(q.shape, generator=gen(5)) * 0.1)
+    q[:, :, 0] = 64.0
+    q[:, 1::2, 0] = -64.0
+    k[..., 0] = 448.0                           # the score's largest part: 448 q0 ks for pages of the one kind
+    for b, n in enumerate(lens.tolist()):
+        pages = table[b, :(n + 15) // 16].tolist()
+        for j, page in enumerate(pages):
+            if (j < len(pages) // 2) == first:
+                k[page, :, :, 0] = -448.0
+                vs[page] *= 2.0 ** (20 + 9 * (j % 7))
+    scale = 40 / (448 * 64 * 2.0 ** -6)         # scores of +-40: probabilities e^-80, 2^-115, of the other kind
+    check_decode(args, softmax_scale=scale)
+    check_decode(args, softmax_scale=scale / 5)
+    check_decode(args, softmax_scale=0.0)
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.3, 1.0, 1e-6])
 def test_decode_softmax_scales(scale):
     check_decode(decode_case(9, [200, 31], 8, 2, 128, 16, torch.bfloat16, E4M3), softmax_scale=scale)
