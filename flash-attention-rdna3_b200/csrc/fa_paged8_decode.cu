@@ -388,7 +388,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint32_t qf[NT][kJ * 4][2];
   float row_scale[NT][2];       // of rows 2 t4, 2 t4 + 1: softmax scale * log2(e) * the query row's own scale
   float o[NT][kNm][4], m[NT][2], l[NT][2];
-  float vref[NT][2];            // powers of two that the columns' products with V are relative to
+  float vinv[NT][2];            // inverses of the powers of two (vref) that the columns' products with V are relative to
+  uint32_t v_limit = 0;         // four times this lane's smallest vref
   int begin_step = 0, stage = 0;
   uint32_t parity = 0;
   for (int u = 0; u < units; ++u) {
@@ -397,6 +398,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // A new item: query rows as fp16 operands. fp16 rows go as they are; a bf16 row is first scaled by the power of
       // two that puts its largest value into [2^14, 2^15), which keeps every bit down to 2^-28 of that value.
       begin_step = at.step;
+      v_limit = 3u << 23;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const int r = chunk0 + nt * 8 + g;
@@ -460,7 +462,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         row_scale[nt][1] = __shfl_sync(0xffffffffu, mine, (2 * t4 + 1) * 4);
         m[nt][0] = m[nt][1] = kNegInf;
         l[nt][0] = l[nt][1] = 0.f;
-        vref[nt][0] = vref[nt][1] = __uint_as_float(1u << 23);
+        vinv[nt][0] = vinv[nt][1] = __uint_as_float(253u << 23);
 #pragma unroll
         for (int i = 0; i < kNm; ++i)
 #pragma unroll
@@ -509,14 +511,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---- Scales and mask. m is a reference, not the maximum: it moves (with everything summed so far) only when a score
     // passes it by more than 2^kSlack, so most tiles need no reduction over the warp. The products with V take p * vs
     // relative to a power of two vref, which is looked at again when m moves or a scale passes it fourfold: what enters
-    // them is below 2^(kSlack + 3), in fp16's range. vref follows the column's largest p * vs, not the scales alone (a large
+    // them is below 2^(kSlack + 2), in fp16's range. vref follows the column's largest p * vs, not the scales alone (a large
     // scale under probabilities next to nothing would push everything else out of fp16's range).
     float v_scale[kMt][2];
     float excess = -1.f;
-    uint32_t v_limit = 0xffffffffu;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) v_limit = min(v_limit, min(__float_as_uint(vref[nt][0]), __float_as_uint(vref[nt][1])));
-    v_limit += 2u << 23;
     bool v_moves = false;
 #pragma unroll
     for (int mt = 0; mt < kMt; ++mt) {
@@ -559,6 +557,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int mt = 0; mt < kMt; ++mt) v_top = fmax3(v_top, fabsf(v_scale[mt][0]), fabsf(v_scale[mt][1]));
       v_top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v_top)));
+      v_limit = 0xffffffffu;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float f[2];
@@ -577,14 +576,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                           fast_exp2(s[mt][nt][2 + e] - z) * fabsf(v_scale[mt][1]));
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) w_top = fmaxf(w_top, __shfl_xor_sync(0xffffffffu, w_top, x));
+          const float vref_old = __uint_as_float((254u << 23) - __float_as_uint(vinv[nt][e]));
           const float alpha = top == m[nt][e] ? 1.f : fast_exp2(m[nt][e] - top);
           // The largest p * vs so far; up to 64 times that where scales are larger, so that ordinary differences between
           // pages do not come back here; and never so far below a scale that their ratio leaves fp32.
-          const float wanted = fmaxf(fmaxf(w_top, alpha * vref[nt][e]), fmaxf(fminf(v_top, 64.f * w_top), 0x1p-100f * v_top));
+          const float wanted = fmaxf(fmaxf(w_top, alpha * vref_old), fmaxf(fminf(v_top, 64.f * w_top), 0x1p-100f * v_top));
           const uint32_t ref = min(max(__float_as_uint(wanted) & 0x7f800000u, 1u << 23), 253u << 23);
-          const int rise = (int)(__float_as_uint(vref[nt][e]) >> 23) - (int)(ref >> 23);
+          const int rise = (int)(__float_as_uint(vref_old) >> 23) - (int)(ref >> 23);
           f[e] = top == m[nt][e] ? __uint_as_float((uint32_t)max(127 + rise, 0) << 23) : fast_exp2(m[nt][e] - top + (float)rise);
-          vref[nt][e] = __uint_as_float(ref);
+          vinv[nt][e] = __uint_as_float((254u << 23) - ref);
+          v_limit = min(v_limit, ref + (2u << 23));
           m[nt][e] = top;
           l[nt][e] *= alpha;
         }
@@ -608,10 +609,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float p10 = fast_exp2(s[mt][nt][2] - z0), p11 = fast_exp2(s[mt][nt][3] - z1);
         l[nt][0] += p00 + p10;
         l[nt][1] += p01 + p11;
-        const float i0 = __uint_as_float((254u << 23) - __float_as_uint(vref[nt][0]));
-        const float i1 = __uint_as_float((254u << 23) - __float_as_uint(vref[nt][1]));
-        b0[nt] = transpose8x8(DType<__half>::pack2(p00 * (v_scale[mt][0] * i0), p01 * (v_scale[mt][0] * i1)));
-        b1[nt] = transpose8x8(DType<__half>::pack2(p10 * (v_scale[mt][1] * i0), p11 * (v_scale[mt][1] * i1)));
+        b0[nt] = transpose8x8(DType<__half>::pack2(p00 * (v_scale[mt][0] * vinv[nt][0]), p01 * (v_scale[mt][0] * vinv[nt][1])));
+        b1[nt] = transpose8x8(DType<__half>::pack2(p10 * (v_scale[mt][1] * vinv[nt][0]), p11 * (v_scale[mt][1] * vinv[nt][1])));
       }
       auto product = [&](int i, uint32_t wa, uint32_t wb, uint32_t wc, uint32_t wd) {
         // four dimensions of tokens ra, rb (and ra + 8, rb + 8): tiles i (dimensions 0, 1) and i + 1 (2, 3)
@@ -693,7 +692,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int x = 4; x < 32; x <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], x);
           top[nt][e] = m[nt][e];
           sum[nt][e] = l[nt][e];
-          weight[nt][e] = vref[nt][e];
+          weight[nt][e] = __uint_as_float((254u << 23) - __float_as_uint(vinv[nt][e]));
         }
       if (warps_head > 1) {  // the warps of a head took its tokens by turns
         if (g == 0)
@@ -712,7 +711,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int w = 0; w < warps_head; ++w) M = fmaxf(M, peer[w * kRows].x);
             const float z = M == kNegInf ? 0.f : M;
             for (int w = 0; w < warps_head; ++w) L += peer[w * kRows].y * fast_exp2(peer[w * kRows].x - z);
-            weight[nt][e] = vref[nt][e] * fast_exp2(m[nt][e] - z);
+            weight[nt][e] *= fast_exp2(m[nt][e] - z);
             top[nt][e] = M;
             sum[nt][e] = L;
           }

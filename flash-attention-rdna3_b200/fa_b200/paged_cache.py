@@ -169,7 +169,8 @@ def paged_kv_append(key, value, k_cache, v_cache, k_scales, v_scales, slot_mappi
     Codes are rounded to nearest, ties to even. Infinities become the largest code, NaN stays NaN (in int8: 0).
 
     The new tokens of a page have to be neighbours in ``slot_mapping`` with slots that rise by one, and a page belongs to
-    one request; `check_status` raises after a call that repeats a slot or goes back inside a page. Inference-only.
+    one request; `check_status` raises after a call in which a token's slot is in the page of the one before it but not the
+    next there. Inference-only.
     """
     if not torch.compiler.is_compiling() and _lib.paged_binding().append(key, value, k_cache, v_cache, k_scales, v_scales,
                                                                          slot_mapping):
