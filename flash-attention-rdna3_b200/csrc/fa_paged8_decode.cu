@@ -39,6 +39,8 @@ constexpr int kStages = 3;
 constexpr int kMaxCtas = 256;
 constexpr int kMergeThreads = 256;
 constexpr float kSlack = 10.f;                  // log2 of what a score may pass the softmax reference by
+constexpr int kTop = 10;                        // log2 of where a column's largest p * vs is put in fp16's range
+constexpr float kRoom = 15.9f;                  // log2 of what p * vs may pass vref by: fp16's largest value, less the error of a log2
 constexpr uint32_t kNoPage = 0x7fffbad0u;       // K scale (a NaN of its own) of tokens whose page id is out of range
 
 struct Args {
@@ -389,16 +391,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   float row_scale[NT][2];       // of rows 2 t4, 2 t4 + 1: softmax scale * log2(e) * the query row's own scale
   float o[NT][kNm][4], m[NT][2], l[NT][2];
   float vinv[NT][2];            // inverses of the powers of two (vref) that the columns' products with V are relative to
-  uint32_t v_limit = 0;         // four times this lane's smallest vref
+  float v_limit = 0.f;          // log2 of this lane's smallest vref, + 127 + kRoom
   int begin_step = 0, stage = 0;
   uint32_t parity = 0;
   for (int u = 0; u < units; ++u) {
     const int head = ((at.item / a.row_chunks) << a.head_shift) + wh, chunk0 = (at.item % a.row_chunks) * kRows;
     if (u == 0 || at.step == 0) {
       // A new item: query rows as fp16 operands. fp16 rows go as they are; a bf16 row is first scaled by the power of
-      // two that puts its largest value into [2^14, 2^15), which keeps every bit down to 2^-28 of that value.
+      // two that puts its largest value into [2^14, 2^15), which keeps every bit down to 2^-31 of that value.
       begin_step = at.step;
-      v_limit = 3u << 23;
+      v_limit = 1.f + kRoom;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const int r = chunk0 + nt * 8 + g;
@@ -510,20 +512,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     // ---- Scales and mask. m is a reference, not the maximum: it moves (with everything summed so far) only when a score
     // passes it by more than 2^kSlack, so most tiles need no reduction over the warp. The products with V take p * vs
-    // relative to a power of two vref, which is looked at again when m moves or a scale passes it fourfold: what enters
-    // them is below 2^(kSlack + 2), in fp16's range. vref follows the column's largest p * vs, not the scales alone (a large
-    // scale under probabilities next to nothing would push everything else out of fp16's range).
-    float v_scale[kMt][2];
-    float excess = -1.f;
-    bool v_moves = false;
+    // relative to a power of two vref, which puts the column's largest p * vs at 2^kTop or above, near the top of fp16's
+    // range: a weight keeps its 11 bits down to 2^-24 of the largest, and what is lost lies below 2^-35 of it, so that many
+    // tokens of small probability count beside one of a large one. vref follows p * vs, not the scales (a large scale under
+    // probabilities next to nothing would push everything else out of the range). Both are looked at again when a score
+    // passes m by too much, and when the lane's largest score and largest scale together could leave the range.
+    float v_scale[kMt][2], v_most = 0.f;
+    float excess = -100.f;  // (so a scale passes vref by less than 2^116, and their ratio stays in fp32)
 #pragma unroll
     for (int mt = 0; mt < kMt; ++mt) {
       const uint32_t at0 = st + mt * 2 * scale8, at1 = at0 + scale8;
       const float k0 = lds_f32(at0), k1 = lds_f32(at1);
       v_scale[mt][0] = lds_f32(at0 + v_scales);
       v_scale[mt][1] = lds_f32(at1 + v_scales);
-      v_moves = v_moves || (__float_as_uint(v_scale[mt][0]) & 0x7fffffffu) >= v_limit ||
-                (__float_as_uint(v_scale[mt][1]) & 0x7fffffffu) >= v_limit;
+      v_most = fmax3(v_most, fabsf(v_scale[mt][0]), fabsf(v_scale[mt][1]));
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -552,12 +554,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int mt = 0; mt < kMt; ++mt) top = fmax3(top, s[mt][nt][e], s[mt][nt][2 + e]);
         excess = fmaxf(excess, top - m[nt][e]);  // (-inf) - (-inf) is NaN, which loses
       }
-    if (__any_sync(0xffffffffu, excess > kSlack || v_moves)) {
-      float v_top = 0.f;
-#pragma unroll
-      for (int mt = 0; mt < kMt; ++mt) v_top = fmax3(v_top, fabsf(v_scale[mt][0]), fabsf(v_scale[mt][1]));
-      v_top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v_top)));
-      v_limit = 0xffffffffu;
+    // (the bits of a positive number, as a number of units of 2^-23, are its log2 + 127 or up to 0.0861 less)
+    const bool leaves = excess + __uint2float_rz(__float_as_uint(v_most)) * 0x1p-23f > v_limit;
+    if (__any_sync(0xffffffffu, excess > kSlack || leaves)) {
+      const float v_top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v_most)));
+      v_limit = INFINITY;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float f[2];
@@ -578,14 +579,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int x = 4; x < 32; x <<= 1) w_top = fmaxf(w_top, __shfl_xor_sync(0xffffffffu, w_top, x));
           const float vref_old = __uint_as_float((254u << 23) - __float_as_uint(vinv[nt][e]));
           const float alpha = top == m[nt][e] ? 1.f : fast_exp2(m[nt][e] - top);
-          // The largest p * vs so far; up to 64 times that where scales are larger, so that ordinary differences between
-          // pages do not come back here; and never so far below a scale that their ratio leaves fp32.
-          const float wanted = fmaxf(fmaxf(w_top, alpha * vref_old), fmaxf(fminf(v_top, 64.f * w_top), 0x1p-100f * v_top));
-          const uint32_t ref = min(max(__float_as_uint(wanted) & 0x7f800000u, 1u << 23), 253u << 23);
+          // 2^-kTop of the largest p * vs so far, and never so far below a scale that their ratio leaves fp32
+          const float wanted = fmaxf(fmaxf(w_top, alpha * vref_old * (float)(1 << kTop)), 0x1p-100f * v_top);
+          const uint32_t ref = (uint32_t)min(max((int)(__float_as_uint(wanted) >> 23) - kTop, 1), 253) << 23;
           const int rise = (int)(__float_as_uint(vref_old) >> 23) - (int)(ref >> 23);
           f[e] = top == m[nt][e] ? __uint_as_float((uint32_t)max(127 + rise, 0) << 23) : fast_exp2(m[nt][e] - top + (float)rise);
           vinv[nt][e] = __uint_as_float((254u << 23) - ref);
-          v_limit = min(v_limit, ref + (2u << 23));
+          v_limit = fminf(v_limit, (float)(ref >> 23) + kRoom);
           m[nt][e] = top;
           l[nt][e] *= alpha;
         }

@@ -91,8 +91,8 @@ def decode8_ref(q, k_cache, v_cache, k_scales, v_scales, block_table, context_le
     """(out, bound) in 64 bits, both (batch, heads_q, dim). `bound` is what a kernel may be off before it rounds its
     output, by arithmetic:
       * p times value scale rounded to fp16 in front of the product with V, relative to a power of two: 2^-11 of each
-        p |v|, and for those below fp16's normal range 2^-25 of that unit. The unit is at most 64 times the row's largest
-        p * scale, at most the largest p times the largest scale, and at least 2^-100 of the latter;
+        p |v|, and for those below fp16's normal range 2^-25 of that unit. The unit is at most 2^-10 of the row's largest
+        p * scale, or 2^-110 of the largest p times the largest scale where that is more;
       * fp32 sums of dim products in the scores: at most (dim / 16 + 8) roundings or truncations of 2^-23 relative to
         sum |q k|, which the exponential turns into that relative error of p, once in the sum and once in its norm;
       * 2^-18 for the exponential and the fp32 sums over tokens (relative to sum p |v|), over at most 2^14 tokens a
@@ -126,6 +126,6 @@ def decode8_ref(q, k_cache, v_cache, k_scales, v_scales, block_table, context_le
             relative = 2.0 ** -11 + 2 * (D / 16 + 8) * 2.0 ** -23 * sums + 2.0 ** -18
             top = 1.0 / torch.exp(s - s.amax(-1, keepdim=True)).sum(-1, keepdim=True)   # p of the largest score
             most = unit[:, h].abs().max() * top
-            step = torch.minimum(most, 64 * (p * unit[:, h].abs()).amax(-1, keepdim=True) + 2.0 ** -100 * most)
+            step = 2.0 ** -10 * torch.maximum((p * unit[:, h].abs()).amax(-1, keepdim=True), 2.0 ** -100 * most)
             bound[b, rows] = relative * weighted + 2.0 ** -25 * step * code[:, h].abs().sum(0)
     return out, bound

@@ -408,6 +408,56 @@ def test_decode_large_value_scales_under_small_probabilities(heads_q, heads_kv, 
     check_decode(args, softmax_scale=0.0)
 
 
+def scored_case(seed, scores, heads_q, heads_kv, dim, dtype, cache):
+    """One request whose token t scores scores[t] in the base-2 exponent (whole numbers from -64 to 63), in every head."""
+    args = decode_case(seed, [len(scores)], heads_q, heads_kv, dim, 16, dtype, cache)
+    q, k, v, ks, vs, table, lens = args
+    q.zero_()
+    q[:, :, :3] = 1.0
+    k.view(torch.uint8).zero_()                 # (zero in both types)
+    high, low = scores // 8 * 4, scores % 8     # high + high + low, each an e4m3 and an int8 value
+    for t, page in enumerate(table[0].tolist()):
+        at = slice(16 * t, 16 * t + 16)
+        n = len(scores[at])
+        for d, part in ((0, high), (1, high), (2, low)):
+            k[page, :n, :, d] = part[at, None].expand(n, heads_kv).to(k.device).float().to(cache)
+    ks.fill_(1.0)
+    vs.fill_(1.0)
+    return args, 0.6931471805599453             # softmax scale ln 2: q . k counts powers of two
+
+
+@pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("heads_q, heads_kv, dim", [(8, 2, 64), (32, 2, 64), (32, 8, 128), (16, 1, 128), (4, 1, 256)])
+@pytest.mark.parametrize("outlier", [1.0, 64.0, 2.0 ** 40])
+@pytest.mark.parametrize("first", [0, 16000])
+def test_decode_many_small_probabilities_beside_a_large_one(cache, heads_q, heads_kv, dim, outlier, first):
+    """A token with next to all of the probability and zeros for values, 16383 others of 2^-20 each that make up the
+    answer, and beside the first a page of larger scale and no probability to speak of (2^-60)."""
+    scores = torch.full((16384,), 0)
+    scores[first], scores[16:32] = 20, -40
+    args, scale = scored_case(30, scores, heads_q, heads_kv, dim, torch.float16, cache)
+    v, vs, table = args[2], args[4], args[5][0].tolist()
+    v.copy_(v.float().abs().to(cache))
+    v.view(torch.uint8)[table[first // 16], first % 16] = 0
+    vs[table[1]] = outlier
+    got = check_decode(args, softmax_scale=scale)
+    assert (got > 0.1).all()
+
+
+@pytest.mark.parametrize("heads_q, heads_kv, dim", [(8, 2, 64), (32, 2, 64), (32, 8, 128), (16, 1, 128), (4, 1, 256)])
+@pytest.mark.parametrize("rise", [3, 5, 9, 11])
+def test_decode_scores_that_rise_from_page_to_page(heads_q, heads_kv, dim, rise):
+    """Scores that climb and fall by `rise` from page to page, below and above what moves the softmax reference, under
+    scales that move the other way or the same way: the weights leave the range of what they are rounded to on both sides."""
+    page = torch.arange(30 * 11) % 30
+    climb = (torch.where(page < 15, page, 29 - page) * rise).clamp(max=120)
+    for sign in (-1, 0, 1):
+        args, scale = scored_case(31, (climb - 60).repeat_interleave(16), heads_q, heads_kv, dim, torch.bfloat16, E4M3)
+        for j, p in enumerate(args[5][0].tolist()):
+            args[4][p] = 2.0 ** (sign * int(climb[j]) / 2)
+        check_decode(args, softmax_scale=scale)
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.3, 1.0, 1e-6])
 def test_decode_softmax_scales(scale):
     check_decode(decode_case(9, [200, 31], 8, 2, 128, 16, torch.bfloat16, E4M3), softmax_scale=scale)
