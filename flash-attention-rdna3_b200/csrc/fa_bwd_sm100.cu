@@ -171,7 +171,10 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   PROF_STAMP(3);
   if (a.compact) {
     const PackedTile pt = find_packed_tile<false>(a.cu_k, a.batch, a.total_k, 128, a.num_tiles, blockIdx.y);
-    if (pt.seq < 0) return;
+    if (pt.seq < 0) {
+      if (a.after_delta) grid_dependency_wait();
+      return;
+    }
     b = pt.seq;
     ktile = pt.tile;
     hk = blockIdx.x;
@@ -179,7 +182,10 @@ bwd_dkdv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     bounded_sequence(a.cu_k, b, a.total_k, &k_start, &Sk);
   }
   const int k0 = ktile * 128;
-  if (k0 >= Sk) return;
+  if (k0 >= Sk) {  // (a grid of such CTAs alone must not end before the delta kernel either, see bwd_dq_kernel)
+    if (a.after_delta) grid_dependency_wait();
+    return;
+  }
   const int tb = a.varlen ? 0 : b;
 
   // 128-query steps that can see this key tile; the mask geometry does not depend on the head
@@ -989,6 +995,10 @@ bwd_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
   tc_fence_before_sync();
   __syncthreads();
   if (warp == 9) tmem_dealloc(tmem_base, 512);
+  // A programmatic dependent that never waits could end before the dK/dV kernel it was launched behind, and a kernel
+  // launched behind this one in the same way (the paged-cache kernels are) would wait for this one alone and write over
+  // q, k, v or dO while dK/dV reads them. So this grid ends after that one; nothing here needs the SM any more.
+  grid_dependency_wait();
   PROF_STAMP(7);
 }
 

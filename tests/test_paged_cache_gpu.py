@@ -721,6 +721,36 @@ def test_captured_behind_copies_and_joined_streams():
                 assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("causal", [False, True])
+def test_append_right_behind_a_backward(monkeypatch, causal):
+    """The recomputing dQ kernel of 16384 queries over 128 keys ends long before the dK/dV kernel that it was let loose
+    beside, which reads the queries to its end: an append that overwrites them comes after both."""
+    from fa_b200 import interface
+
+    monkeypatch.setattr(interface, "DS_WORKSPACE_LIMIT_BYTES", 0)
+    heads, sq, dim = 4, 16384, 128
+    g = gen(1)
+    q0, k, v, dout = (torch.randn(1, heads, n, dim, generator=g).half().cuda() for n in (sq, 128, 128, sq))
+    x = torch.randn(sq, 8, dim, generator=g).half().cuda()
+    slots = torch.arange(sq, device="cuda")
+    other = torch.empty(sq // 16, 16, 8, dim, dtype=torch.int8, device="cuda")
+    scales = torch.ones(2, sq // 16, 8, device="cuda")
+    got = []
+    for append in (False, True, True, True):
+        q = q0.clone()
+        over = q.view(torch.int8).view(sq // 16, 16, 8, dim)     # the queries' memory as a cache of 8-bit pages
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        out = fa_b200.flash_attention(*leaves, causal=causal)
+        grads = torch.autograd.grad(out, leaves, dout)
+        if append:
+            fa_b200.paged_kv_append(x, x, over, other, *scales, slots)
+            torch.cuda.synchronize()
+            assert not torch.equal(q, q0)
+        got.append(grads)
+    for grads in got[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(grads, got[0]))
+
+
 @pytest.mark.parametrize("skip", [0, 4])
 def test_decode_lost_wait_sets_the_status_word(skip):
     """The loading warp leaves a unit out, so that bounded waits run out on both sides; the kernel ends by itself, what it
