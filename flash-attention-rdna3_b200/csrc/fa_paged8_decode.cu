@@ -125,12 +125,15 @@ __device__ __forceinline__ int clamped_len(const Args& a, int b) {
   return (int)max((int64_t)0, min((int64_t)a.lens[b * a.cl_stride], (int64_t)a.max_blocks << a.shift));
 }
 
+// Units that `len` tokens take. (Lengths go up to 2^31 - 1: here and below, nothing is added to one in 32 bits.)
+__device__ __forceinline__ int steps_of(int len, int span) { return (int)(((uint32_t)len + span - 1) / (uint32_t)span); }
+
 // Place in the line of units: request, item of it, step of the item.
 struct Cursor {
   int b, item, step, steps, len;
   __device__ __forceinline__ void enter(const Args& a, int span) {
     len = clamped_len(a, b);
-    steps = (len + span - 1) / span;
+    steps = steps_of(len, span);
   }
   __device__ __forceinline__ void advance(const Args& a, int span, int items) {
     if (++step < steps) return;
@@ -209,8 +212,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   {
     const int per = (a.batch + kWarps * 32 - 1) / (kWarps * 32), b0 = min(tid * per, a.batch), b1 = min(b0 + per, a.batch);
     const int len0 = b0 < b1 ? clamped_len(a, b0) : 0;  // (the only one of this thread up to 256 requests)
-    int64_t mine = (int64_t)((len0 + span - 1) / span) * items;
-    for (int b = b0 + 1; b < b1; ++b) mine += (int64_t)((clamped_len(a, b) + span - 1) / span) * items;
+    int64_t mine = (int64_t)steps_of(len0, span) * items;
+    for (int b = b0 + 1; b < b1; ++b) mine += (int64_t)steps_of(clamped_len(a, b), span) * items;
     int64_t sum = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -241,7 +244,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (u_begin < u_end && at <= u_begin && u_begin < sum) {
       for (int b = b0; b < b1; ++b) {
         const int len = b == b0 ? len0 : clamped_len(a, b);
-        const int64_t n = (int64_t)((len + span - 1) / span) * items;
+        const int64_t n = (int64_t)steps_of(len, span) * items;
         if (at <= u_begin && u_begin < at + n) {
           start_s[0] = b;
           start_s[1] = at;
@@ -257,7 +260,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (units > 0) {
     at.b = (int)start_s[0];
     at.len = (int)start_s[2];
-    at.steps = (at.len + span - 1) / span;
+    at.steps = steps_of(at.len, span);
     const int64_t rest = u_begin - start_s[1];
     if (rest < INT32_MAX) {
       at.item = (int)rest / at.steps;
@@ -274,15 +277,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     // (the CTA was launched with 168 registers a thread: 56 + 2 * 224 = 3 * 168)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp > kWarps) return;
-    const int box = 1 << a.box_shift, boxes = span >> a.box_shift, in_page = (1 << a.shift) - 1;
+    const int box = 1 << a.box_shift, boxes = span >> a.box_shift, page_mask = (1 << a.shift) - 1;
     const int entries = (span >> a.scale_shift) << a.head_shift;
     const uint32_t box_bytes = (uint32_t)(box << (a.head_shift - T::kPair)) * kRow;
-    auto page_at = [&](const Cursor& c, int pos) -> int {
-      if (pos >= c.len) return -1;
-      const int id = a.table[c.b * a.bt_sb + (pos >> a.shift) * a.bt_sk];
+    auto page_at = [&](const Cursor& c, int off) -> int {  // page of the off-th token of the step
+      const int pos0 = c.step * span;
+      if (off >= c.len - pos0) return -1;
+      const int id = a.table[c.b * a.bt_sb + ((pos0 + off) >> a.shift) * a.bt_sk];
       return id >= 0 && id < a.num_blocks ? id : -1;
     };
-    auto fetch = [&](const Cursor& c) -> int { return lane < boxes ? page_at(c, c.step * span + lane * box) : -1; };
+    auto fetch = [&](const Cursor& c) -> int { return lane < boxes ? page_at(c, lane * box) : -1; };
     int page = -1;
     if (units > 0) page = fetch(at);
     int stage = 0, issued = 0;
@@ -298,21 +302,22 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       bool plain = true;
       for (int i = lane; i < boxes && issued != a.skip_unit; i += 32) {
-        const int pos = pos0 + i * box, id = i < 32 ? page : page_at(at, pos);
-        plain = plain && id >= 0 && pos + box <= at.len;
+        const int off = i * box, id = i < 32 ? page : page_at(at, off);
+        const int in_page = ((pos0 & page_mask) + off) & page_mask;  // (pos0 + off may pass 2^31)
+        plain = plain && id >= 0 && off + box <= at.len - pos0;
         // tokens behind the context and pages out of range: a page behind the last one, which reads as zeros
         const int c3 = id >= 0 ? id : a.num_blocks;
 #pragma unroll
         for (int h = 0; h < T::kHalves; ++h) {
-          tma_load_4d(kt + h * kHalfBytes + i * box_bytes, &k_map, &full_s[stage], h * 128, pos & in_page, head0 >> T::kPair, c3);
-          tma_load_4d(kt + kStageBytes / 2 + h * kHalfBytes + i * box_bytes, &v_map, &full_s[stage], h * 128, pos & in_page, head0 >> T::kPair, c3);
+          tma_load_4d(kt + h * kHalfBytes + i * box_bytes, &k_map, &full_s[stage], h * 128, in_page, head0 >> T::kPair, c3);
+          tma_load_4d(kt + kStageBytes / 2 + h * kHalfBytes + i * box_bytes, &v_map, &full_s[stage], h * 128, in_page, head0 >> T::kPair, c3);
         }
       }
       plain = __all_sync(0xffffffffu, plain);
       for (int e0 = 0; e0 < entries; e0 += 32) {
-        const int e = e0 + lane, pos = pos0 + ((e >> a.head_shift) << a.scale_shift);
-        int id = __shfl_sync(0xffffffffu, page, ((pos - pos0) >> a.box_shift) & 31);
-        if (boxes > 32) id = page_at(at, pos);
+        const int e = e0 + lane, off = (e >> a.head_shift) << a.scale_shift;
+        int id = __shfl_sync(0xffffffffu, page, (off >> a.box_shift) & 31);
+        if (boxes > 32) id = page_at(at, off);
         if (e >= entries) continue;
         const uint32_t k_to = st + e * 4, v_to = k_to + entries * 4;
         const int head = head0 + (e & (heads_cta - 1));
@@ -476,7 +481,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool plain = plain_s[stage] != 0;
     const uint32_t kt = head_at + stage * kStageBytes, vt = kt + kStageBytes / 2;
     const uint32_t st = scale_base + stage * Smem<D, NT>::kScaleStage;
-    const int left = at.len - (at.step * span + wt * kTokens);  // tokens of the context from this tile's first on
+    const int left = at.len - at.step * span - wt * kTokens;  // tokens of the context from this tile's first on
     if (!lost) {
     // ---- scores: rows are tokens, columns query heads
     float s[kMt][NT][4];

@@ -540,6 +540,31 @@ def test_decode_offsets_beyond_32_bits():
         assert bytes_equal(big[-1:].contiguous(), little)
 
 
+@pytest.mark.parametrize("heads_kv, dim, last", [(1, 16, 16), (1, 16, 1), (2, 64, 9)])
+def test_decode_contexts_up_to_the_last_32_bit_length(heads_kv, dim, last):
+    """2^27 - 1 rows of the table that all name one page, and a request of ordinary length behind: the answer is that of
+    the one page (the last row holds `last` tokens, which at 2^-27 of the sum do not show). The longest running sums are
+    2^31 / 148 / 256 units long with up to four additions a unit, each off by 2^-24 in the sum of the probabilities and by
+    2^-23 in that of the products: together 4.1 % of sum p |v| at most. The values are positive, so that shows zeros and
+    whatever lay in the output's memory before."""
+    drift = 4 * 1.5 * 2.0 ** -23 * 2.0 ** 31 / 148 / 256
+    args = decode_case(40, [16, 77], 4 * heads_kv, heads_kv, dim, 16, torch.bfloat16, torch.int8)
+    q, k, v, ks, vs, table, lens = args
+    v.copy_(v.float().abs().clamp(min=1).to(torch.int8))
+    want, _ = oracle.decode8_ref(*args)
+    width = 2 ** 27 - 1
+    far = table[:1, :1].expand(1, width)
+    lens[0] = (width - 1) * 16 + last
+    got = fa_b200.flash_attention_decode_paged_8bit(q[:1], k, v, ks, vs, far, lens[:1])
+    assert ((got.double() - want[:1]).abs() <= (drift + 2.0 ** -7) * want[:1]).all()
+    # in a batch: a request of ordinary length in front and one behind (all rows of the table name their first page)
+    ends, page = torch.tensor([1, 0, 1], device="cuda"), torch.stack((table[1, 0], table[0, 0], table[1, 0]))
+    want = oracle.decode8_ref(q[ends], k, v, ks, vs, page[:, None], ints([13, 16, 16]))[0]
+    got = fa_b200.flash_attention_decode_paged_8bit(q[ends], k, v, ks, vs, page[:, None].expand(3, width),
+                                                    torch.stack((lens[0] * 0 + 13, lens[0], lens[0] * 0 + 1600)))
+    assert ((got.double() - want).abs() <= (drift + 2.0 ** -7) * want).all()
+
+
 # ---------------------------------------------------------------------------------------------------
 # together
 # ---------------------------------------------------------------------------------------------------
