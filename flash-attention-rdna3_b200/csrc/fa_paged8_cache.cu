@@ -214,14 +214,15 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanArgs
         a.slots[t0 + 32 * k + lane] = id[k] >= 0 && id[k] < a.num_blocks ? ((int64_t)id[k] << a.shift) + offset[k] : -1;
   }
   // block-table entries of the new pages, and the places of the stack above its old top
-  for (int p0 = first - lane; p0 < taken; p0 += step) {
-    const int p = min(p0 + lane, taken - 1);
-    const int b = lane_first_above(need_end, a.batch, warp_first_above(need_end, a.batch, p0), p);
+  // (counted in 64 bits: a stack may hold up to 2^31 - 1 pages, and the last step leads past that)
+  for (int64_t p0 = first - lane; p0 < taken; p0 += step) {
+    const int p = (int)min(p0 + lane, (int64_t)taken - 1);
+    const int b = lane_first_above(need_end, a.batch, warp_first_above(need_end, a.batch, (int)p0), p);
     const int have = (int)((len[b] + round_up) >> a.shift);
     if (p0 + lane < taken)
       a.table[(int64_t)b * a.bt_stride + have + (p - (b > 0 ? need_end[b - 1] : 0))] = *entry(available - 1 - p);
   }
-  for (int p = count + first; p < min(left, a.num_blocks); p += step) a.stack[p] = *entry(p);
+  for (int64_t p = (int64_t)count + first; p < min(left, a.num_blocks); p += step) a.stack[p] = *entry((int)p);
   for (int b = first; b < a.batch; b += step) {
     const int begin = b > 0 ? cu_end[b - 1] : 0;
     a.cu[b + 1] = cu_end[b];

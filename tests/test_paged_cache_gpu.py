@@ -106,6 +106,27 @@ def test_plan_strange_values():
     torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("inplace", [False, True])
+def test_plan_of_the_largest_stack(inplace):
+    """A stack of 2^31 - 1 places that is full but for ten: pages come back up to its last place, and a step that pops
+    from there. (Only the top of the stack is looked at; the pool behind it need not exist for planning.)"""
+    places = 2 ** 31 - 1
+    stack = torch.empty(places, dtype=torch.int32, device="cuda")
+    stack[-60:] = torch.arange(60, dtype=torch.int32, device="cuda")
+    table = torch.full((600, 4), -1, dtype=torch.int32, device="cuda")
+    table[5, :4], table[400, :2] = ints([2 ** 31 - 2, 7, 8, 9]), ints([1000, 11])
+    lens, new = torch.zeros(2, 600, dtype=torch.int32, device="cuda")
+    lens[5], lens[400], new[5], new[400] = 60, 20, -1, -1
+    new[500], new[501] = 40, 17                 # three pages and two, popped from the ones that have just come back
+    count = ints([places - 10])
+    slots, cu, after, left = fa_b200.paged_kv_plan(lens, new, table, stack, count, 57, 16, inplace=inplace)
+    assert int(left) == places - 10 + 6 - 5
+    assert table[500].tolist() == [11, 1000, 9, -1] and table[501].tolist() == [8, 7, -1, -1]
+    assert stack[-10:].tolist() == [2 ** 31 - 2] + list(range(51, 60))
+    assert slots[:16].tolist() == list(range(176, 192)) and slots[-1] == 7 * 16
+    assert after.nonzero().flatten().tolist() == [500, 501]
+
+
 def test_plan_strided_inputs():
     lens, new, table, stack, count, tokens = random_plan(21, 25, 16, 9, 30, 60)
     wide = torch.full((25, 31), -9, dtype=torch.int32, device="cuda")
