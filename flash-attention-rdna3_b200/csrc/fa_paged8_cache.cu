@@ -3,6 +3,7 @@
 #include "fa_paged8.cuh"
 #include "fa_sm100.cuh"
 
+#include <atomic>
 #include <type_traits>
 
 namespace fa {
@@ -533,6 +534,25 @@ int check_launch(const char* what, cudaError_t e) {
   return e == cudaSuccess ? 0 : set_error(FA_ERR_LAUNCH, "%s launch failed: %s", what, cudaGetErrorString(e));
 }
 
+// The shared memory of the largest batch, allowed once a device and never lowered: calls of other threads may be on their
+// way to a launch.
+constexpr int kPlanBytes = 17;  // shared memory of a request
+constexpr int kMaxDevices = 64;
+template <int kTogether> int allow_plan_smem() {
+  static std::atomic<bool> allowed[kMaxDevices];
+  int dev = -1;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && dev < kMaxDevices && allowed[dev].load(std::memory_order_relaxed)) return 0;
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(paged_plan_kernel<kTogether>, cudaFuncAttributeMaxDynamicSharedMemorySize, FA_PLAN_MAX_BATCH * kPlanBytes);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return set_error(FA_ERR_LAUNCH, "plan: cannot get %d bytes of shared memory: %s", FA_PLAN_MAX_BATCH * kPlanBytes, cudaGetErrorString(e));
+  }
+  if (dev < kMaxDevices) allowed[dev].store(true, std::memory_order_relaxed);
+  return 0;
+}
+
 }  // namespace
 
 int launch_paged_plan(const fa_paged_plan_params& p, cudaStream_t stream) {
@@ -557,14 +577,10 @@ int launch_paged_plan(const fa_paged_plan_params& p, cudaStream_t stream) {
   a.lens_out = p.context_lens_out;
   a.count_out = p.free_count_out;
   const bool inplace = a.lens_out == a.lens || a.count_out == a.count;
-  const int smem = p.batch * 17;
+  const int smem = p.batch * kPlanBytes;
   if (smem > 40 * 1024) {
-    const cudaError_t e = inplace ? cudaFuncSetAttribute(paged_plan_kernel<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)
-                                  : cudaFuncSetAttribute(paged_plan_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) {
-      cudaGetLastError();
-      return set_error(FA_ERR_LAUNCH, "plan: cannot get %d bytes of shared memory: %s", smem, cudaGetErrorString(e));
-    }
+    const int rc = inplace ? allow_plan_smem<4>() : allow_plan_smem<1>();
+    if (rc) return rc;
   }
   // A thread for each request or token of a decode step; more CTAs for prompts, as many as there are groups of tokens for
   // where the lengths are not updated in place, a cluster that takes four groups at a time where they are.

@@ -127,6 +127,42 @@ def test_plan_of_the_largest_stack(inplace):
     assert after.nonzero().flatten().tolist() == [500, 501]
 
 
+def test_plans_of_large_batches_from_two_threads():
+    """C callers hold no lock: plans of different batches, both above what shared memory a kernel has unasked, are launched
+    side by side, and none takes from another what it needs."""
+    import ctypes
+    import threading
+
+    from fa_b200 import _lib
+
+    lib, wrong = _lib.load(), []
+
+    def caller(batch):
+        torch.cuda.set_device(0)
+        lens, new = torch.zeros(2, batch, dtype=torch.int32, device="cuda")
+        table = torch.zeros(batch, 2, dtype=torch.int32, device="cuda")
+        stack, count = torch.zeros(4, dtype=torch.int32, device="cuda"), ints([4])
+        cu, lens_out = torch.empty(batch + 1, dtype=torch.int32, device="cuda"), torch.empty_like(lens)
+        count_out = torch.empty_like(count)
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        p = _lib.PagedPlanParams(batch, 2, 4, 16, 0, lens.data_ptr(), 1, new.data_ptr(), 1, table.data_ptr(), 2,
+                                 stack.data_ptr(), count.data_ptr(), None, cu.data_ptr(), lens_out.data_ptr(),
+                                 count_out.data_ptr())
+        for _ in range(1500):
+            rc = lib.fa_paged_plan(ctypes.byref(p), ctypes.c_void_p(stream.cuda_stream))
+            if rc:
+                wrong.append(rc)
+        stream.synchronize()
+
+    threads = [threading.Thread(target=caller, args=(n,)) for n in (8192, 2500, 8000, 3000)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
 def test_plan_strided_inputs():
     lens, new, table, stack, count, tokens = random_plan(21, 25, 16, 9, 30, 60)
     wide = torch.full((25, 31), -9, dtype=torch.int32, device="cuda")
