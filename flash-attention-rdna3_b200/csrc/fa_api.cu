@@ -231,6 +231,8 @@ int32_t fa_paged_plan(const fa_paged_plan_params* p, void* stream) {
     return fa::set_error(FA_ERR_INVALID_ARGUMENT, "plan: no pointer may be NULL");
   if (p->batch > 1 && p->bt_stride < p->max_blocks)
     return fa::set_error(FA_ERR_INVALID_ARGUMENT, "plan: rows of the block table must not overlap");
+  if (p->context_lens_out == p->context_lens && p->batch > 1 && p->cl_stride != 1)
+    return fa::set_error(FA_ERR_INVALID_ARGUMENT, "plan: context_lens must be contiguous to be updated in place");
   return fa::launch_paged_plan(*p, static_cast<cudaStream_t>(stream));
 }
 

@@ -239,8 +239,8 @@ enum fa_cache_dtype { FA_CACHE_E4M3 = 0, FA_CACHE_INT8 = 1 };
      3. slot_mapping[t] = page * block_size + offset of every new token; -1 for the tokens of requests that are not
         served and behind the last token. The block table gets the new pages; entries past them stay as they were.
      4. context_lens_out = L + n (served), 0 (ended), L (not served); free_count_out = what the stack holds after it.
-   context_lens_out and free_count_out may be the inputs themselves. Where they are not, a second call with the same
-   inputs gives the same results. Page ids outside [0, num_blocks) give slot -1. */
+   context_lens_out and free_count_out may be the inputs themselves (context_lens then with a stride of 1: its place is
+   written densely). Where they are not, a second call with the same inputs gives the same results. Page ids outside [0, num_blocks) give slot -1. */
 typedef struct fa_paged_plan_params {
   int32_t batch, max_blocks, num_blocks, block_size;
   int64_t num_tokens;             /* entries of slot_mapping */

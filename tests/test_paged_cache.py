@@ -154,6 +154,21 @@ def test_c_entries_refuse_without_a_gpu():
         assert lib.fa_paged8_append(ctypes.byref(_lib.Paged8AppendParams(**{**append, **bad})), None) < 0, bad
 
 
+def test_c_plan_refuses_strided_lengths_in_place():
+    """The kernel reads context_lens with its stride and writes context_lens_out densely: as one tensor they need stride 1."""
+    lib = _lib.load()
+    x = (ctypes.c_int64 * 64)()
+    at, other = ctypes.addressof(x), ctypes.addressof(x) + 256
+    plan = dict(batch=2, max_blocks=4, num_blocks=4, block_size=16, num_tokens=1, context_lens=at, new_lens=at, nl_stride=1,
+                block_table=at, bt_stride=4, free_blocks=at, free_count=at, slot_mapping=at, cu_seqlens=at,
+                free_count_out=at)
+    assert lib.fa_paged_plan(ctypes.byref(_lib.PagedPlanParams(**plan, cl_stride=2, context_lens_out=at)), None) == -1
+    assert b"contiguous" in lib.fa_last_error_string()
+    if not torch.cuda.is_available():               # (addresses of host memory: nothing is launched without a device)
+        for kw in (dict(cl_stride=2, context_lens_out=other), dict(cl_stride=1, context_lens_out=at)):
+            assert lib.fa_paged_plan(ctypes.byref(_lib.PagedPlanParams(**plan, **kw)), None) != -1
+
+
 def test_struct_sizes_match_the_header():
     src = ('#include "fa_b200.h"\n#include <stdio.h>\n#include <stddef.h>\nint main(void){'
            'printf("%zu %zu %zu %zu %zu %d %d", sizeof(fa_paged_plan_params), sizeof(fa_paged8_append_params), '
