@@ -15,6 +15,7 @@
 #include <torch/csrc/utils/pybind.h>
 
 #include <cmath>
+#include <initializer_list>
 #include <optional>
 #include <stdexcept>
 #include <string>
@@ -75,6 +76,13 @@ bool rows16(const at::Tensor& t) {
 
 int dtype_of(const at::Tensor& t) {
   return t.scalar_type() == at::kHalf ? FA_F16 : t.scalar_type() == at::kBFloat16 ? FA_BF16 : -1;
+}
+
+bool needs_grad(std::initializer_list<const at::Tensor*> tensors) {
+  if (!c10::GradMode::is_enabled()) return false;
+  for (const at::Tensor* t : tensors)
+    if (t->requires_grad()) return true;
+  return false;
 }
 
 struct Cache {
@@ -189,7 +197,7 @@ bool append(py::handle key, py::handle value, py::handle k_cache, py::handle v_c
   for (const at::Tensor* t : {c.ks, c.vs})
     for (int i = 0; i < 2; ++i)
       if (t->size(i) > 1 && t->stride(i) <= 0) return false;
-  if (c10::GradMode::is_enabled() && (k->requires_grad() || v->requires_grad())) return false;
+  if (needs_grad({k, v, c.k, c.v, c.ks, c.vs})) return false;
   fa_paged8_append_params p = {};
   p.dtype = dtype_of(*k);
   p.cache_dtype = c.dtype;
@@ -234,7 +242,7 @@ py::object decode(py::handle query, py::handle k_cache, py::handle v_cache, py::
       heads % c.k->size(2) || table->size(0) != batch || lens->size(0) != batch || table->size(1) <= 0 ||
       table->size(1) > INT32_MAX || !rows16(*q))
     return py::none();
-  if (c10::GradMode::is_enabled() && q->requires_grad()) return py::none();
+  if (needs_grad({q, c.k, c.v, c.ks, c.vs})) return py::none();
   fa_paged8_params p = {};
   p.dtype = dtype_of(*q);
   p.cache_dtype = c.dtype;

@@ -176,7 +176,7 @@ def paged_kv_append(key, value, k_cache, v_cache, k_scales, v_scales, slot_mappi
                                                                          slot_mapping):
         return
     validate_paged8_append_inputs(key, value, k_cache, v_cache, k_scales, v_scales, slot_mapping)
-    validate_inference_only(key, value)
+    validate_inference_only(key, value, k_cache, v_cache, k_scales, v_scales)
     if _direct(key):
         _append_impl(key, value, k_cache, v_cache, k_scales, v_scales, slot_mapping)
     else:
@@ -247,7 +247,7 @@ def flash_attention_decode_paged_8bit(query, k_cache, v_cache, k_scales, v_scale
         if out is not None:
             return out
     validate_paged8_inputs(query, k_cache, v_cache, k_scales, v_scales, block_table, context_lens)
-    validate_inference_only(query)
+    validate_inference_only(query, k_cache, v_cache, k_scales, v_scales)
     validate_softmax_scale(softmax_scale)
     softmax_scale = 1.0 / math.sqrt(query.shape[2]) if softmax_scale is None else float(softmax_scale)
     impl = _decode8_impl if _direct(query) else _decode8_op

@@ -127,6 +127,22 @@ def test_other_refusals():
                 call(*args)
 
 
+@pytest.mark.parametrize("index", range(5))
+def test_inference_only_whatever_needs_the_gradient(monkeypatch, index):
+    """Scales (and e4m3 caches) are floating tensors too: no gradient would reach them, so the calls refuse."""
+    from fa_b200 import _validation
+
+    monkeypatch.setattr(_validation, "_require_platform", lambda device: None)
+    args = decode_args()
+    args[index].requires_grad_(True)
+    with pytest.raises(RuntimeError, match="inference-only"):
+        fa_b200.flash_attention_decode_paged_8bit(*args)
+    args = append_args()
+    args[index + 1].requires_grad_(True)            # value, caches, scales
+    with pytest.raises(RuntimeError, match="inference-only"):
+        fa_b200.paged_kv_append(*args)
+
+
 def test_c_entries_refuse_without_a_gpu():
     lib = _lib.load()
     for fn, cls in ((lib.fa_paged_plan, _lib.PagedPlanParams), (lib.fa_paged8_append, _lib.Paged8AppendParams),

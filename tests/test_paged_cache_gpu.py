@@ -754,6 +754,26 @@ def test_inference_only():
         fa_b200.flash_attention_decode_paged_8bit(*d)
 
 
+@pytest.mark.parametrize("index", range(5))
+def test_inference_only_for_caches_and_scales(index):
+    d = decode_case(20, [40], 8, 2, 64, 16, torch.float16, E4M3)
+    x = inputs(3, 4, 2, 64, torch.float16)
+    slots = torch.arange(4, device="cuda")
+    fa_b200.flash_attention_decode_paged_8bit(*d)        # (the compiled binding takes over behind the first call)
+    fa_b200.paged_kv_append(x, x, *d[1:5], slots)
+    before = [t.clone() for t in d[1:5]]
+    d[index].requires_grad_(True)
+    with pytest.raises(RuntimeError, match="inference-only"):
+        fa_b200.flash_attention_decode_paged_8bit(*d)
+    if index > 0:
+        with pytest.raises(RuntimeError, match="inference-only"):
+            fa_b200.paged_kv_append(x * 2, x, *d[1:5], slots)
+        assert all(bytes_equal(a.detach(), b) for a, b in zip(d[1:5], before))
+    with torch.no_grad():
+        fa_b200.flash_attention_decode_paged_8bit(*d)
+        fa_b200.paged_kv_append(x, x, *d[1:5], slots)
+
+
 def test_captured_behind_copies_and_joined_streams():
     """The kernels start early behind whatever precedes them: a copy, a fill, a kernel of another stream, in a graph and
     outside, never before it has written what they read."""
