@@ -45,6 +45,12 @@ def _direct(t):
         return False
 
 
+def _rows16(t):
+    """`t`, or a copy of it whose rows can be read with 16-byte loads (a tensor that begins off such a boundary may be
+    contiguous all the same)."""
+    return t if _vector_friendly(t) else t.clone(memory_format=torch.contiguous_format)
+
+
 def _call(fn, params, device):
     """Launch on torch's current stream of `device`, whichever device is current."""
     if torch.cuda.current_device() == device.index:
@@ -135,8 +141,7 @@ def _append_impl(key, value, k_cache, v_cache, k_scales, v_scales, slot_mapping)
         return
     lib = _lib.load()
     device = key.device
-    key = key if _vector_friendly(key) else key.contiguous()
-    value = value if _vector_friendly(value) else value.contiguous()
+    key, value = _rows16(key), _rows16(value)
     p = _lib.Paged8AppendParams(
         _DTYPE_CODE[key.dtype], _CACHE_CODE[k_cache.dtype], key.shape[1], key.shape[2], k_cache.shape[0],
         k_cache.shape[1], key.shape[0], key.data_ptr(), key.stride(), value.data_ptr(), value.stride(),
@@ -201,7 +206,7 @@ def _decode8_impl(query, k_cache, v_cache, k_scales, v_scales, block_table, cont
     device = query.device
     batch, heads_q, head_dim = query.shape
     blocks, block_size, heads_kv, _ = k_cache.shape
-    query = query if _vector_friendly(query) else query.contiguous()
+    query = _rows16(query)
     out = torch.empty((batch, heads_q, head_dim), dtype=query.dtype, device=device)
     nbytes = _workspace_bytes(device.index, batch, heads_q, heads_kv, head_dim, block_size)
     workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)

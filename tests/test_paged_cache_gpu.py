@@ -560,6 +560,28 @@ def test_decode_strided(cache, dim):
     assert torch.equal(fa_b200.flash_attention_decode_paged_8bit(odd, *args[1:]), want)
 
 
+def test_contiguous_rows_off_a_16_byte_boundary():
+    """Queries, keys and values that are contiguous but begin 2 or 8 bytes into memory are copied, not refused."""
+    args = decode_case(12, [100, 333], 8, 4, 64, 16, torch.bfloat16, E4M3)
+    want = check_decode(args)
+    x = inputs(3, 5, 4, 64, torch.bfloat16)
+    slots = torch.arange(16, 21, device="cuda")
+    caches = [[t.clone() for t in args[1:5]] for _ in range(2)]
+    fa_b200.paged_kv_append(x, -x, *caches[0], slots)
+    for skip in (1, 4):
+        def shifted(t):
+            out = torch.empty(t.numel() + skip, dtype=t.dtype, device="cuda")[skip:].view(t.shape)
+            assert out.is_contiguous() and out.data_ptr() % 16
+            return out.copy_(t)
+
+        assert torch.equal(fa_b200.flash_attention_decode_paged_8bit(shifted(args[0]), *args[1:]), want)
+        fa_b200.paged_kv_append(shifted(x), shifted(-x), *caches[1], slots)
+        assert all(bytes_equal(a, b) for a, b in zip(*caches))
+    with pytest.raises(RuntimeError, match="16-byte"):      # caches are never copied
+        k = torch.empty(args[1].numel() + 8, dtype=torch.uint8, device="cuda")[8:].view(E4M3).view(args[1].shape)
+        fa_b200.flash_attention_decode_paged_8bit(args[0], k, *args[2:])
+
+
 def test_decode_one_page_for_many_requests():
     """A prefix that requests share: the same page in several rows, and twice in one."""
     args = decode_case(13, [64, 64, 64], 8, 2, 128, 16, torch.float16, E4M3)
