@@ -174,8 +174,9 @@ def paged_kv_append(key, value, k_cache, v_cache, k_scales, v_scales, slot_mappi
     Codes are rounded to nearest, ties to even. Infinities become the largest code, NaN stays NaN (in int8: 0).
 
     The new tokens of a page have to be neighbours in ``slot_mapping`` with slots that rise by one, and a page belongs to
-    one request; `check_status` raises after a call in which a token's slot is in the page of the one before it but not the
-    next there. Inference-only.
+    one request: what a page holds is unspecified otherwise (other pages are as they should be). `check_status` raises
+    after a call in which a token's slot is in the page of the one before it but not the next there; tokens of a page that
+    lie apart, with other tokens or ones without a slot between them, are not noticed. Inference-only.
     """
     if not torch.compiler.is_compiling() and _lib.paged_binding().append(key, value, k_cache, v_cache, k_scales, v_scales,
                                                                          slot_mapping):

@@ -339,6 +339,23 @@ def test_append_reports_slots_out_of_order(slots):
         assert bytes_equal(t[1:].contiguous(), u)
 
 
+@pytest.mark.parametrize("slots", [[5, -1, 6, 17, 33], [5, 20, 6], [20, 5, 33, 4], list(range(16)) + [-1] * 300 + [3, 17]])
+@pytest.mark.parametrize("bs, dim", [(16, 64), (16, 256), (256, 128)])
+def test_append_leaves_other_pages_alone_when_tokens_of_one_lie_apart(slots, bs, dim):
+    """Nothing is promised for page 0, and nothing else is touched."""
+    slots = [s if s < 16 else s // 16 * bs + s % 16 for s in slots]
+    x = inputs(3, len(slots), 2, dim, torch.float16)
+    k, ks = filled_cache(1, 4, bs, 2, dim, E4M3)
+    v, vs = filled_cache(2, 4, bs, 2, dim, torch.int8)[0].view(E4M3), ks * 2
+    # the tokens of the other pages, by themselves
+    others = [i for i, s in enumerate(slots) if s >= bs]
+    want = [oracle.append_ref(y[others], c, s, [slots[i] for i in others]) for y, c, s in ((x, k, ks), (-x, v, vs))]
+    fa_b200.paged_kv_append(x, -x, k, v, ks, vs, torch.tensor(slots, device="cuda"))
+    for c, s, (codes, scales) in ((k, ks, want[0]), (v, vs, want[1])):
+        assert torch.equal(s[1:].double(), scales[1:])
+        assert torch.equal(torch.nan_to_num(c[1:].double(), nan=1e9), torch.nan_to_num(codes[1:], nan=1e9))
+
+
 # ---------------------------------------------------------------------------------------------------
 # decode
 # ---------------------------------------------------------------------------------------------------
