@@ -1,10 +1,12 @@
 """Build libfa_b200.so (the C-ABI CUDA library) in-tree with nvcc for sm_100a.
 
-Usage: python flash-attention-rdna3_b200/build.py [--force] [--verbose] [--prof] [--debug-bounds]
+Usage: python flash-attention-rdna3_b200/build.py [--force] [--verbose] [--prof] [--debug-bounds] [--no-binding]
 
 Each .cu file is compiled to an object only when it or a header is newer than the object, then all
 objects are linked into fa_b200/libfa_b200.so next to the Python package that loads it. g++ then builds
-fa_b200/_paged_native.so, the Python binding of the paged-cache calls.
+fa_b200/_paged_native.so, the Python binding of the paged-cache calls, against the installed PyTorch (and again when that
+or Python has changed). The library needs neither: without PyTorch, or with --no-binding, it is all that is built, and C
+callers have everything.
 
 --prof builds a second library, fa_b200/libfa_b200_prof.so, with -DFA_PROF: the tensor-core forward, backward and decode
 kernels then count, per CTA and role, the cycles spent in each phase of their loops (csrc/fa_prof.cuh) and the library
@@ -44,7 +46,7 @@ def _newest_header():
     return max(os.path.getmtime(p) for p in paths)
 
 
-def build(force=False, verbose=False, prof=False, debug_bounds=False):
+def build(force=False, verbose=False, prof=False, debug_bounds=False, binding=True):
     global OBJ, OUT
     if prof:
         OBJ = os.path.join(HERE, "build", "prof")
@@ -84,24 +86,39 @@ def build(force=False, verbose=False, prof=False, debug_bounds=False):
         if r.returncode != 0:
             sys.stderr.write(r.stdout + r.stderr)
             raise RuntimeError("link failed")
-    if not prof and not debug_bounds:
+    if binding and not prof and not debug_bounds:
         _build_binding(force, verbose, header_time)
     return OUT
 
 
+def _built_for(path):
+    """What the binding was last built against, as _build_binding wrote it down."""
+    try:
+        with open(path) as f:
+            return f.read()
+    except OSError:
+        return ""
+
+
 def _build_binding(force, verbose, header_time):
     """The Python binding of the paged-cache calls (csrc/fa_paged8_bind.cpp), a module against torch's C++ headers."""
-    src = os.path.join(CSRC, "fa_paged8_bind.cpp")
-    if not force and os.path.exists(BINDING) and os.path.getmtime(BINDING) >= max(os.path.getmtime(src), header_time):
+    try:
+        import torch
+    except ImportError:
+        sys.stderr.write("PyTorch is not installed: fa_b200/_paged_native.so, which only Python needs, is not built\n")
         return
     import sysconfig
 
-    import torch
+    src = os.path.join(CSRC, "fa_paged8_bind.cpp")
+    stamp, against = os.path.join(OBJ, "_paged_native.txt"), f"torch {torch.__version__}, {sysconfig.get_config_var('SOABI')}"
+    fresh = os.path.exists(BINDING) and os.path.getmtime(BINDING) >= max(os.path.getmtime(src), header_time)
+    if not force and fresh and _built_for(stamp) == against:
+        return
     from torch.utils import cpp_extension
 
     lib = os.path.join(os.path.dirname(torch.__file__), "lib")
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++20", "-shared", "-fPIC", "-fvisibility=hidden", src, "-o", BINDING,
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f'-DFA_TORCH="{torch.__version__}"',
            f"-I{sysconfig.get_paths()['include']}",
            *(f"-isystem{d}" for d in cpp_extension.include_paths("cuda")), f"-L{lib}",
            "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-Wl,--as-needed"]
@@ -109,9 +126,11 @@ def _build_binding(force, verbose, header_time):
     if verbose or r.returncode != 0:
         sys.stderr.write(f"--- fa_paged8_bind.cpp\n{r.stdout}{r.stderr}\n")
     if r.returncode != 0:
-        raise RuntimeError("compiling fa_paged8_bind.cpp failed")
+        raise RuntimeError("compiling fa_paged8_bind.cpp failed (--no-binding leaves it out: only Python needs it)")
+    with open(stamp, "w") as f:
+        f.write(against)
 
 
 if __name__ == "__main__":
     print(build(force="--force" in sys.argv, verbose="--verbose" in sys.argv, prof="--prof" in sys.argv,
-                debug_bounds="--debug-bounds" in sys.argv))
+                debug_bounds="--debug-bounds" in sys.argv, binding="--no-binding" not in sys.argv))

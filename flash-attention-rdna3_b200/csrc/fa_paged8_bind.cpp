@@ -285,6 +285,7 @@ py::object decode(py::handle query, py::handle k_cache, py::handle v_cache, py::
 }  // namespace
 
 PYBIND11_MODULE(_paged_native, m) {
+  m.attr("torch_version") = FA_TORCH;  // its headers are compiled in
   m.def("bind", &bind);
   m.def("set_status", &set_status);
   m.def("plan", &plan);

@@ -230,6 +230,15 @@ def load():
 _binding = None
 
 
+def _check_binding(module):
+    """The binding has torch's headers compiled in: another version's tensors may lie differently in memory."""
+    import torch
+
+    if module.torch_version != torch.__version__:
+        raise RuntimeError(f"fa_b200: {BINDING_PATH} is built for PyTorch {module.torch_version} and this is "
+                           f"{torch.__version__}: run `python flash-attention-rdna3_b200/build.py` again")
+
+
 def paged_binding():
     """The compiled binding of the paged-cache calls (csrc/fa_paged8_bind.cpp), bound to the loaded library."""
     global _binding
@@ -245,8 +254,13 @@ def paged_binding():
             import importlib.util
 
             spec = importlib.util.spec_from_file_location("_paged_native", BINDING_PATH)
-            module = importlib.util.module_from_spec(spec)
-            spec.loader.exec_module(module)
+            try:
+                module = importlib.util.module_from_spec(spec)
+                spec.loader.exec_module(module)
+            except ImportError as e:
+                raise RuntimeError(f"fa_b200: {BINDING_PATH} does not load ({e}); it may be built for another PyTorch: "
+                                   "run `python flash-attention-rdna3_b200/build.py` again") from e
+            _check_binding(module)
             module.bind(*(C.cast(getattr(lib, name), C.c_void_p).value for name in (
                 "fa_paged_plan", "fa_paged8_append", "fa_decode_paged8", "fa_workspace_bytes", "fa_last_error_string")))
             _binding = module

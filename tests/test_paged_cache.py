@@ -185,6 +185,55 @@ def test_c_plan_refuses_strided_lengths_in_place():
             assert lib.fa_paged_plan(ctypes.byref(_lib.PagedPlanParams(**plan, **kw)), None) != -1
 
 
+def build_module():
+    import importlib.util
+
+    path = os.path.join(ROOT, "flash-attention-rdna3_b200", "build.py")
+    spec = importlib.util.spec_from_file_location("fa_b200_build_module", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    return module
+
+
+def test_the_library_builds_without_torch(monkeypatch, capsys, tmp_path):
+    """Only the Python binding needs PyTorch: without it the build ends with the library and says so."""
+    import sys
+
+    build = build_module()
+    monkeypatch.setattr(build, "BINDING", str(tmp_path / "binding.so"))
+    monkeypatch.setitem(sys.modules, "torch", None)                 # import torch raises ImportError
+    assert build.build() == build.OUT
+    assert "not built" in capsys.readouterr().err and not os.path.exists(build.BINDING)
+    monkeypatch.setattr(build, "_build_binding", lambda *a: pytest.fail("built"))
+    assert build.build(binding=False) == build.OUT
+
+
+def test_the_binding_is_built_again_for_another_torch(monkeypatch):
+    build = build_module()
+    build.build()
+    ran = []
+
+    def compiler(cmd, **kw):
+        ran.append(cmd)
+        return subprocess.CompletedProcess(cmd, 1, "", "")
+
+    monkeypatch.setattr(build.subprocess, "run", compiler)
+    build.build()                                                   # all is up to date
+    assert not ran
+    monkeypatch.setattr(torch, "__version__", "2.8.0")
+    with pytest.raises(RuntimeError, match="no-binding"):
+        build.build()
+    assert len(ran) == 1 and '-DFA_TORCH="2.8.0"' in ran[0]
+
+
+def test_a_binding_of_another_torch_is_refused(monkeypatch):
+    module = _lib.paged_binding()
+    _lib._check_binding(module)
+    monkeypatch.setattr(torch, "__version__", "2.8.0")
+    with pytest.raises(RuntimeError, match="built for PyTorch"):
+        _lib._check_binding(module)
+
+
 def test_struct_sizes_match_the_header():
     src = ('#include "fa_b200.h"\n#include <stdio.h>\n#include <stddef.h>\nint main(void){'
            'printf("%zu %zu %zu %zu %zu %d %d", sizeof(fa_paged_plan_params), sizeof(fa_paged8_append_params), '
