@@ -5,6 +5,17 @@
 
 namespace fa {
 
+// A result rounded towards zero and what it lacks of the exact one: rounded to odd. The last bit of a result that is not
+// exact is 1 then, so that rounding it again to a code is rounding the exact one once.
+__device__ __forceinline__ float to_odd(float towards_zero, float rest) {
+  return __uint_as_float(__float_as_uint(towards_zero) | (fabsf(rest) > 0.f ? 1u : 0u));
+}
+
+__device__ __forceinline__ float odd_product(float x, float y) {
+  const float p = __fmul_rz(x, y);
+  return to_odd(p, fmaf(x, y, -p));
+}
+
 // e4m3: 1 sign, 4 exponent (bias 7), 3 mantissa bits; largest finite value 448 = 1.75 * 2^8, code 0x7f is NaN.
 // int8: -127 .. 127. Every e4m3 and every int8 value is an fp16 value, so codes become fp16 without rounding.
 struct CodeE4M3 {
@@ -36,6 +47,10 @@ struct CodeE4M3 {
     unpack_f32x2(x, &a, &b);
     unpack_f32x2(y, &c, &d);
     return pack4(a, b, c, d);
+  }
+  // older codes under a new scale: times the ratio of the two
+  __device__ static __forceinline__ uint32_t pack4_codes(float2 lo, float2 hi, float ratio) {
+    return pack4(odd_product(lo.x, ratio), odd_product(lo.y, ratio), odd_product(hi.x, ratio), odd_product(hi.y, ratio));
   }
   // fp16 pairs times a power of two: exact, or below fp16's normal range, where every code is 0 (half of the smallest is 2^-10)
   __device__ static __forceinline__ uint32_t pack4_half(__half2 lo, __half2 hi, __half2 f) {
@@ -76,6 +91,13 @@ struct CodeInt8 {
     unpack_f32x2(y, &c, &d);
     return __byte_perm(__byte_perm(__float_as_uint(a), __float_as_uint(b), 0x0040),
                        __byte_perm(__float_as_uint(c), __float_as_uint(d), 0x0040), 0x5410);
+  }
+  // Older codes under a new scale: the product is exact inside the fused addition. (A code of -128, which only the caller
+  // can have written, becomes -127 at least; ratios above 1 only come from a scale that was no positive number.)
+  __device__ static __forceinline__ uint32_t pack4_codes(float2 lo, float2 hi, float ratio) {
+    if (!(fabsf(ratio) <= 1.f))
+      return pack4(odd_product(lo.x, ratio), odd_product(lo.y, ratio), odd_product(hi.x, ratio), odd_product(hi.y, ratio));
+    return __vmaxs4(pack4_times(lo.x, lo.y, hi.x, hi.y, ratio), 0x81818181u);
   }
   // The same in fp16, whose 1.5 * 2^10 + x has a last bit of 1 too: the product is exact inside the fused addition
   __device__ static __forceinline__ uint32_t pack4_half(__half2 lo, __half2 hi, __half2 f) {

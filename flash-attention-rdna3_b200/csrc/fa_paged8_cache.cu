@@ -309,10 +309,18 @@ __device__ __forceinline__ uint32_t scaled4(uint32_t lo, uint32_t hi, float inve
   const float2 x = DType<T>::unpack2(lo), y = DType<T>::unpack2(hi);
   return C8::pack4_times(x.x, x.y, y.x, y.y, inverse);
 }
+__device__ __forceinline__ float divided(float x, float scale) {
+  if (scale < 0x1p-60f) {  // (the rest of a division by a tiny scale would be below fp32's range)
+    x *= 0x1p60f;
+    scale *= 0x1p60f;
+  }
+  const float q = __fdiv_rz(x, scale);
+  return to_odd(q, fmaf(-q, scale, x));
+}
 template <typename T, typename C8>
 __device__ __noinline__ uint32_t divided4(uint32_t lo, uint32_t hi, float scale) {
   const float2 x = DType<T>::unpack2(lo), y = DType<T>::unpack2(hi);
-  return C8::pack4(__fdiv_rn(x.x, scale), __fdiv_rn(x.y, scale), __fdiv_rn(y.x, scale), __fdiv_rn(y.y, scale));
+  return C8::pack4(divided(x.x, scale), divided(x.y, scale), divided(y.x, scale), divided(y.y, scale));
 }
 
 template <typename T, typename C8, bool kWide>
@@ -475,7 +483,7 @@ __global__ void __launch_bounds__(kAppendThreads, 3) paged8_append_kernel(const 
 
     // ---- older tokens of the page, when its scale has grown
     if (offset > 0 && scale != old) {
-      const float ratio = __fdiv_rn(old, scale);
+      const float ratio = __fdiv_rn(old, scale);  // (exact: the scale has grown to a power of two)
       const int r8 = lane / lanes8, c8 = lane % lanes8;
       for (int j = sub * rows8 + r8; r8 < rows8 && j < offset; j += warps * rows8) {
         uint4* at = reinterpret_cast<uint4*>(page_base + j * a.c_st[kv] + c8 * 16);
@@ -484,7 +492,7 @@ __global__ void __launch_bounds__(kAppendThreads, 3) paged8_append_kernel(const 
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const float2 lo = DType<__half>::unpack2(C8::lo(w[k])), hi = DType<__half>::unpack2(C8::hi(w[k]));
-          w[k] = C8::pack4(lo.x * ratio, lo.y * ratio, hi.x * ratio, hi.y * ratio);
+          w[k] = C8::pack4_codes(lo, hi, ratio);
         }
         *at = v;
       }

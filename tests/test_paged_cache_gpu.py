@@ -339,6 +339,69 @@ def test_append_reports_slots_out_of_order(slots):
         assert bytes_equal(t[1:].contiguous(), u)
 
 
+@pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("heads, dim, bs, runs", [
+    # few tokens of many heads: one warp for runs of up to four times what it holds
+    (8, 128, 64, [(3, 0, 64), (0, 5, 59), (6, 0, 64), (None, 0, 2), (2, 60, 4), (1, 0, 7)]),
+    (16, 256, 32, [(3, 0, 32), (0, 9, 23), (4, 0, 25), (1, 31, 1), (2, 0, 32)]),
+    # several warps a run
+    (2, 128, 256, [(1, 3, 253), (0, 0, 200), (None, 0, 1), (3, 255, 1), (2, 0, 16), (4, 100, 17)]),
+    (1, 16, 1024, [(0, 0, 600), (1, 1000, 24), (2, 0, 1024), (4, 7, 3)])])
+def test_append_runs_longer_than_the_registers_and_special_values(cache, dtype, heads, dim, bs, runs):
+    """Infinities, NaN, zeros, the smallest and the largest numbers in runs that a warp reads twice and in runs that several
+    warps share, over pages whose scales are no powers of two."""
+    slots = runs_to_slots(runs, bs)
+    n = slots.numel()
+    for special in (False, True):
+        k, ks = filled_cache(1, 7, bs, heads, dim, cache)
+        v, vs = filled_cache(2, 7, bs, heads, dim, cache)
+        x, y = inputs(3, n, heads, dim, dtype), inputs(4, n, heads, dim, dtype)
+        if special:
+            ks.mul_(1.37)
+            vs[::2].mul_(2.0 ** 9)
+            x[n // 3, 0, 5], x[n // 2, -1, 0], x[n - 1, 0, dim - 1] = float("inf"), float("-inf"), float("nan")
+            x[runs[0][2] - 1, -1, 3] = float("nan")
+            y[:runs[0][2]] = 0
+            y[n // 2:] *= 2.0 ** -10
+            y[-3:-1] = torch.finfo(dtype).max
+        check_append(x, y, k, v, ks, vs, slots)
+
+
+@pytest.mark.parametrize("dim, bs", [(64, 16), (128, 256)])
+@pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_append_rounds_once_under_any_scale(cache, dtype, dim, bs):
+    """Quotients and products within 2^-25 of a tie between two codes, on either side: rounded to fp32 first they would be
+    ties. Scales 1.37 * 2^i, 2^i (1 + 2^-22), 2^i (2 - 2^-22); every code as an older one, and new values next to every tie."""
+    half = bs // 2
+    for n, scale in enumerate(m * 2.0 ** i for i in (-70, -2, 0, 9) for m in (1.37, 1 + 2.0 ** -22, 2 - 2.0 ** -22)):
+        if cache == torch.int8:
+            codes = torch.arange(bs * dim) % 255 - 127
+            mids = torch.arange(half * dim) % 254 - 126.5
+        else:
+            codes = torch.arange(bs * dim) % 254
+            codes = torch.where(codes < 127, codes, codes + 1).to(torch.uint8).view(E4M3)
+            finite = torch.arange(127, dtype=torch.uint8).view(E4M3).float()
+            mids = torch.cat(((finite[1:] + finite[:-1]) / 2, -(finite[1:] + finite[:-1]) / 2))
+            mids = mids[torch.arange(half * dim) % len(mids)]
+        k = codes.to(torch.int8).view(1, bs, 1, dim).cuda() if cache == torch.int8 else codes.view(1, bs, 1, dim).cuda()
+        ks = torch.full((1, 1), scale, dtype=torch.float32, device="cuda")
+        x = (mids.double() * ks.item()).view(half, 1, dim).to(dtype).cuda()       # stays under the page's scale
+        slots = torch.arange(half, bs, device="cuda")
+        if torch.isfinite(x).all() and x.abs().max() > 0:
+            check_append(x, -x, k.clone(), k.clone(), ks.clone(), ks.clone(), slots)
+        # and one value that makes the scale grow by 2, 4, 8; where the old one was negative, the new one may be smaller
+        for grow in (1.2, 3.0, 7.0, -0.01, -0.6, -3.0):
+            if grow < 0 and n % 3:
+                continue
+            x = torch.zeros(1, 1, dim, dtype=dtype, device="cuda")
+            x[0, 0, 0] = grow * oracle.LARGEST[cache] * ks.item()
+            if x[0, 0, 0].isfinite():
+                old = ks if grow > 0 else -ks
+                check_append(x, -x, k.clone(), k.clone(), old.clone(), old.clone(), slots[:1])
+
+
 @pytest.mark.parametrize("slots", [[5, -1, 6, 17, 33], [5, 20, 6], [20, 5, 33, 4], list(range(16)) + [-1] * 300 + [3, 17]])
 @pytest.mark.parametrize("bs, dim", [(16, 64), (16, 256), (256, 128)])
 def test_append_leaves_other_pages_alone_when_tokens_of_one_lie_apart(slots, bs, dim):
