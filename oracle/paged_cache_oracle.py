@@ -39,9 +39,10 @@ def plan_ref(context_lens, new_lens, block_table, free_blocks, free_count, num_t
             if 0 <= page < capacity:
                 slots[begin + i] = page * block_size + (L + i) % block_size
         out_lens.append(L + n)
-    for i in range(int(free_count), len(held)):  # what lies above the old top is written; popped places stay
+    left = min(len(held), capacity)             # (pages that return to a full stack are lost)
+    for i in range(int(free_count), left):      # what lies above the old top is written; popped places stay
         stack[i] = held[i]
-    return slots, cu, out_lens, len(held), table, stack
+    return slots, cu, out_lens, left, table, stack
 
 
 def round_codes(x, dtype):

@@ -107,6 +107,26 @@ def test_plan_strange_values():
 
 
 @pytest.mark.parametrize("inplace", [False, True])
+@pytest.mark.parametrize("given, meant", [(10 ** 9, None), (-5, 0), (2 ** 31 - 1, None), (-2 ** 31, 0)])
+@pytest.mark.parametrize("ends", [0.0, 0.3, 1.0])
+def test_plan_counts_outside_the_stack(given, meant, ends, inplace):
+    """A count outside the stack is taken for a full or an empty one; neither the table nor the stack is written outside."""
+    lens, new, table, stack, _, tokens = random_plan(12, 40, 16, 8, 40, 60, ends=ends)
+    meant = stack.numel() if meant is None else meant
+    want = oracle.plan_ref(lens.tolist(), new.tolist(), table.cpu(), stack.cpu(), meant, tokens, 16)
+    wide, long = torch.full((44, 14), -9, dtype=torch.int32, device="cuda"), ints([-9] * (stack.numel() + 512))
+    t, s = wide[2:42, 3:11], long[256:-256]
+    t.copy_(table)
+    s.copy_(stack)
+    got = fa_b200.paged_kv_plan(lens, new, t, s, ints([given]), tokens, 16, inplace=inplace)
+    for name, a, b in zip(("slots", "cu", "lens", "count", "table", "stack"), (*got[:3], got[3][0], t, s), want):
+        assert a.tolist() == b, name
+    t.fill_(-9)
+    s.fill_(-9)
+    assert (wide == -9).all() and (long == -9).all()
+
+
+@pytest.mark.parametrize("inplace", [False, True])
 def test_plan_of_the_largest_stack(inplace):
     """A stack of 2^31 - 1 places that is full but for ten: pages come back up to its last place, and a step that pops
     from there. (Only the top of the stack is looked at; the pool behind it need not exist for planning.)"""
@@ -400,6 +420,21 @@ def test_append_rounds_once_under_any_scale(cache, dtype, dim, bs):
             if x[0, 0, 0].isfinite():
                 old = ks if grow > 0 else -ks
                 check_append(x, -x, k.clone(), k.clone(), old.clone(), old.clone(), slots[:1])
+
+
+@pytest.mark.parametrize("slots", [[5, 5], [6, 5], [3, 7], list(range(8, 16)) + [15] * 40, [9] * 400])
+@pytest.mark.parametrize("dim, bs", [(128, 256), (64, 1024)])
+def test_append_reports_slots_out_of_order_in_large_pages(slots, dim, bs):
+    k, ks = filled_cache(1, 3, bs, 2, dim, E4M3)
+    v, vs = filled_cache(2, 3, bs, 2, dim, E4M3)
+    x = inputs(3, len(slots), 2, dim, torch.float16)
+    other = [t[1:].clone() for t in (k, v, ks, vs)]
+    fa_b200.paged_kv_append(x, x, k, v, ks, vs, torch.tensor(slots, device="cuda"))
+    with pytest.raises(RuntimeError, match="repeat or do not rise"):
+        fa_b200.check_status()
+    fa_b200.check_status()
+    for t, u in zip((k, v, ks, vs), other):
+        assert bytes_equal(t[1:].contiguous(), u)
 
 
 @pytest.mark.parametrize("slots", [[5, -1, 6, 17, 33], [5, 20, 6], [20, 5, 33, 4], list(range(16)) + [-1] * 300 + [3, 17]])
