@@ -185,7 +185,13 @@ def _status_word(device):
         key = torch.cuda.current_device()
     word = _status_words.get(key)
     if word is None:
-        word = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", key))
+        # Never set to zero on a stream that is being captured: each replay would do it again, and wipe out what other
+        # calls have reported. (The word may lie in that graph's memory: it is never freed.)
+        with torch.cuda.device(key):
+            word = torch.empty(1, dtype=torch.int32, device=torch.device("cuda", key))
+            side = torch.cuda.Stream() if torch.cuda.is_current_stream_capturing() else torch.cuda.current_stream()
+            with torch.cuda.stream(side):
+                word.zero_()
         _status_words[key] = word
     return word
 

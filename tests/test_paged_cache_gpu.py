@@ -846,6 +846,51 @@ def test_steps_captured_in_a_graph():
     assert bytes_equal(live.k_cache, ref.k_cache) and torch.equal(live.k_scales, ref.k_scales)
 
 
+FIRST_CALLS_CAPTURED = """
+import sys
+sys.path[:0] = {path!r}
+import torch, fa_b200
+g = torch.Generator().manual_seed(1)
+key, value, q = (torch.randn(2, n, 64, generator=g).half().cuda() for n in (2, 2, 8))
+x = [fa_b200.PagedKVCache8(1, 30, 16, 2, 64, 2, 10) for _ in range(2)]
+new = torch.ones(2, dtype=torch.int32, device="cuda")
+junk = torch.full((1 << 22,), 0x55, dtype=torch.uint8, device="cuda")      # what the allocator hands out next is not zero
+del junk
+
+def step(c):
+    slots, _ = c.plan(new, 2)
+    c.append(0, key, value, slots)
+    return c.decode(0, q)
+
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = step(x[0])
+fa_b200.check_status()                      # nothing has run yet, and nothing is reported
+for _ in range(3):
+    graph.replay()
+    assert torch.equal(out, step(x[1]))
+fa_b200.check_status()
+# a report of another call is not wiped out by a replay
+caches = [t[0] for t in (x[1].k_cache, x[1].v_cache, x[1].k_scales, x[1].v_scales)]
+fa_b200.paged_kv_append(key, value, *caches, torch.tensor([5, 5], device="cuda"))
+graph.replay()
+try:
+    fa_b200.check_status()
+except RuntimeError as e:
+    assert "repeat" in str(e), e
+    print("reported")
+"""
+
+
+def test_the_first_calls_of_a_process_may_be_captured():
+    import subprocess
+    import sys
+
+    r = subprocess.run([sys.executable, "-c", FIRST_CALLS_CAPTURED.format(path=[p for p in sys.path if p])],
+                       capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "reported" in r.stdout, r.stdout[-500:] + r.stderr[-1500:]
+
+
 def test_two_streams_at_once():
     a = decode_case(16, [9000, 50], 32, 8, 128, 16, torch.float16, E4M3)
     b = decode_case(17, [400] * 40, 32, 8, 128, 16, torch.float16, E4M3)
@@ -1014,6 +1059,13 @@ def test_plan_of_the_largest_batches():
     assert args[5] > 350000
     check_plan(args, 16)
     check_plan(random_plan(43, 300, 16, 400, 3000, 40000, ends=0.1), 16, inplace=True)
+
+
+def test_plan_of_the_largest_batch_in_place():
+    check_plan(random_plan(41, 8192, 16, 24, 40, 60000), 16, inplace=True)
+    args = random_plan(44, 8192, 64, 24, 1, 8000, ends=0.1)
+    for _ in range(3):                          # steps that go on from one another
+        check_plan(args, 64, inplace=True)
 
 
 @pytest.mark.parametrize("cache", CACHES)
