@@ -1,6 +1,6 @@
 // Python binding of the paged 8-bit cache's three entry points for the calls that a server makes for every token and layer.
-// A call of this module takes 2 to 3 us on the host where the same checks, tensors and ctypes structure take 21 us in
-// Python; with kernels of 3 to 10 us that is what a decode step costs.
+// A call of this module takes 4 us on the host for an append, 6 to 7 for a plan and 8 for a decode, where the same checks,
+// tensors and ctypes structure take 20 to 33 us in Python; with kernels of 3 to 10 us that is what a decode step costs.
 //
 // Each function looks at its arguments and either launches and returns the result, or returns None without having done
 // anything. None means "not this way": tensors that break a contract (Python then finds and names it), that need a copy

@@ -21,8 +21,9 @@ int log2_of(int x) {
 // Everything follows from three running sums over the requests (new tokens, pages that come back, pages needed): every
 // CTA forms them for itself in shared memory, and tokens and pages then find their request there. Where the lengths are
 // updated in place the CTAs are one cluster, whose barrier separates the reads of the lengths from the writes. Bound by
-// latency (lengths, sums, ids, slots: three trips to memory): 4.4 us for a decode step of 64 requests, 7.8 us for 65613
-// tokens of 256 requests (23.5 us with one cluster of eight CTAs and a bisection for every token).
+// latency (lengths, sums, ids, slots: three trips to memory): 4.4 us for a decode step of 64 requests, 7.9 us for 65613
+// tokens of 256 requests (23.5 us with one cluster of eight CTAs and a bisection for every token; updated in place, in one
+// cluster, they take 3.2 times as long as in 128 CTAs).
 constexpr int kPlanThreads = 512;
 constexpr int kPlanMaxCluster = 8;
 constexpr int kPlanMaxCtas = 128;
@@ -241,8 +242,8 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanArgs
 // A task is the run of new tokens of one page, for one head, of keys or of values. Its rows stay in registers between
 // the maximum and the rounding (up to 8 loads of 16 bytes a lane and `warps` warps a task; longer runs are read twice).
 // A CTA holds 8 / warps tasks of the same runs: the heads of a token are neighbours in memory. Bound by memory with many
-// tokens, but only where few instructions go to a value: 45 us for 32704 tokens of 16 heads of 64, fp16 -> int8 (201 MB,
-// 4.4 TB/s, 68 % of a plain copy's rate), 14 us for 8192 tokens of 8 heads of 128, bf16 -> e4m3 (50 MB, 3.6 TB/s); 13
+// tokens, but only where few instructions go to a value: 45.5 us for 32704 tokens of 16 heads of 64, fp16 -> int8 (201 MB,
+// 4.4 TB/s, 67 % of a plain copy's rate), 14 us for 8192 tokens of 8 heads of 128, bf16 -> e4m3 (50 MB, 3.6 TB/s); 13
 // instructions a value before the folded maxima and the 16-bit arithmetic: 64 and 18 us. A decode step of 128 requests
 // takes 4 us. 80 registers hold the rows and leave 24 warps an SM; reading them again instead (64 or 40 registers) takes
 // 59 and 78 us.

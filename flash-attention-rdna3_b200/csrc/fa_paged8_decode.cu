@@ -17,9 +17,10 @@
 // workspace, and paged8_merge_kernel joins the parts in the order of the stretches.
 //
 // Measured on a B200 (both kernels, device time): 64 requests of 1 - 16381 tokens, 32/8 heads of 128: 167 us for 1.075 GB
-// (6.46 TB/s, 98 % of a plain copy's rate); 4 x 16384 tokens: 33 us (4.0 TB/s): 3 us until the first boxes are asked for,
-// 5 - 6 us until the first tile is there (the ring of all SMs, 28 MB, is on its way), 1.47 us a tile, up to 3 us between the
-// first and the last SM, 4 us for the merge; 1 x 256 tokens: 8 us. With one copy loop a warp (cp.async, no producer) the
+// in a replayed graph (6.46 TB/s, 98 % of a plain copy's rate; call by call, with inputs that alternate, 174 - 186 us);
+// 4 x 16384 tokens: 33.5 us (4.0 TB/s): 3 us until the first boxes are asked for, 5 - 6 us until the first tile is there (the
+// ring of all SMs, 28 MB, is on its way), 1.47 us a tile, up to 3 us between the first and the last SM, 4 us for the merge;
+// 1 x 256 tokens: 7.5 us. With one copy loop a warp (cp.async, no producer) the
 // first takes 197 us; with two CTAs an SM and half tiles 291 us; with one head a CTA (boxes of 2 KB) 268 us.
 #include <cuda.h>
 
