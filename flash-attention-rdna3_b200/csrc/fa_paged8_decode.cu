@@ -722,12 +722,23 @@ __global__ void __launch_bounds__(kThreads, 1)
             sum[nt][e] = L;
           }
       }
-      if (whole)
+      // A whole item is divided by its sum; a part by the sum's power of two, which moves into m (p reaches 2^kSlack, and the
+      // sum of many of it times large values would leave fp32).
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) weight[nt][e] = sum[nt][e] == 0.f ? 0.f : weight[nt][e] / sum[nt][e];
-      else if (wt == 0 && g == 0)
+        for (int e = 0; e < 2; ++e) {
+          if (whole) {
+            weight[nt][e] = sum[nt][e] == 0.f ? 0.f : weight[nt][e] / sum[nt][e];
+          } else {
+            const uint32_t power = sum[nt][e] == 0.f ? 127u << 23 : __float_as_uint(sum[nt][e]) & 0x7f800000u;
+            const float inverse = __uint_as_float((254u << 23) - power);
+            weight[nt][e] *= inverse;
+            sum[nt][e] *= inverse;
+            top[nt][e] += (float)((int)(power >> 23) - 127);
+          }
+        }
+      if (!whole && wt == 0 && g == 0)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll

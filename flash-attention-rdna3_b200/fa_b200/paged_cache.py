@@ -241,11 +241,12 @@ def flash_attention_decode_paged_8bit(query, k_cache, v_cache, k_scales, v_scale
     `paged_kv_append` fills.
 
     query ``(batch, q_heads, head_dim)`` float16 or bfloat16 (head_dim 16, 32, 64, 128 or 256); caches and scales as in
-    the module's description, any fp32 scales; ``block_table`` int32 ``(batch, max_blocks_per_seq)``; ``context_lens``
+    the module's description, any finite fp32 scales; ``block_table`` int32 ``(batch, max_blocks_per_seq)``; ``context_lens``
     int32 ``(batch,)``, clamped to the table. Pages out of range contribute nothing and an empty context gives zeros.
     Products and sums are fp32 over fp16 operands. Keys and values are exact in fp16; probability times value scale is
     rounded to it, off by 2^-11 of itself or by 2^-35 of its row's largest, whichever is more; bf16 queries are exact
-    down to 2^-31 of the row's largest value, and off by at most 2^-39 of that below. Non-causal, inference-only.
+    down to 2^-31 of the row's largest value, and off by at most 2^-39 of that below. Values (code times scale) up to 2^117
+    leave no sum's range. Non-causal, inference-only.
     """
     if not torch.compiler.is_compiling():
         out = _lib.paged_binding().decode(query, k_cache, v_cache, k_scales, v_scales, block_table, context_lens,

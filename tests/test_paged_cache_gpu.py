@@ -580,6 +580,23 @@ def test_decode_large_value_scales_under_small_probabilities(heads_q, heads_kv, 
     check_decode(args, softmax_scale=0.0)
 
 
+@pytest.mark.parametrize("heads_q, heads_kv, dim", [(8, 2, 64), (32, 2, 64), (16, 8, 128), (5, 1, 256), (12, 3, 32)])
+@pytest.mark.parametrize("lens", [[40, 3], [700, 9000], [30000], [300] * 50])
+@pytest.mark.parametrize("cache", CACHES)
+def test_decode_values_near_the_largest_numbers(heads_q, heads_kv, dim, lens, cache):
+    """Values up to 2^117 under scores that rise above what the softmax started from: every sum that is kept in between
+    stays in fp32's range."""
+    args = decode_case(32, lens, heads_q, heads_kv, dim, 16, torch.bfloat16, cache)
+    args[1].copy_((args[1].float() / 4).to(cache))
+    args[4].copy_(torch.exp2(torch.randint(85, 111 if cache == torch.int8 else 109, args[4].shape, generator=gen(6)).float()))
+    for b in range(len(lens)):                  # keys that grow along the context
+        pages = args[5][b][args[5][b] >= 0].long()
+        args[3][pages] *= torch.linspace(0.1, 4, len(pages), device="cuda")[:, None]
+    largest = (args[2].double().abs().amax((1, 3)) * args[4].double()).max()
+    assert 2.0 ** 105 < largest <= 2.0 ** 117   # (short contexts meet few of the large scales)
+    check_decode(args)
+
+
 def scored_case(seed, scores, heads_q, heads_kv, dim, dtype, cache):
     """One request whose token t scores scores[t] in the base-2 exponent (whole numbers from -64 to 63), in every head."""
     args = decode_case(seed, [len(scores)], heads_q, heads_kv, dim, 16, dtype, cache)
@@ -628,6 +645,18 @@ def test_decode_scores_that_rise_from_page_to_page(heads_q, heads_kv, dim, rise)
         for j, p in enumerate(args[5][0].tolist()):
             args[4][p] = 2.0 ** (sign * int(climb[j]) / 2)
         check_decode(args, softmax_scale=scale)
+
+
+@pytest.mark.parametrize("cache, power", [(E4M3, 108), (torch.int8, 110)])
+@pytest.mark.parametrize("heads_q, heads_kv, dim, tokens", [(32, 8, 128, 16384), (8, 8, 256, 9000), (32, 2, 64, 100000)])
+def test_decode_large_values_under_scores_above_the_reference(cache, power, heads_q, heads_kv, dim, tokens):
+    """Tiles whose scores pass the ones before them by 2^9, just under what moves the softmax reference, over values of one
+    sign up to 2^117: what a part of the context hands in is 2^9 times some hundred such values."""
+    scores = 9 * (torch.arange(tokens) // 256 % 3 > 0)
+    args, scale = scored_case(33, scores, heads_q, heads_kv, dim, torch.bfloat16, cache)
+    args[2].copy_(args[2].float().abs().to(cache))
+    args[4].fill_(2.0 ** power)
+    assert check_decode(args, softmax_scale=scale).min() > 2.0 ** (power + 3)
 
 
 @pytest.mark.parametrize("scale", [0.0, -0.3, 1.0, 1e-6])
